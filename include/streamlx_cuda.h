@@ -42,6 +42,7 @@ extern "C" {
 #define SLX_ERR_RANGE (-9)           /* device: an operand outside the range
                                         a kernel computes exactly (fp16
                                         operands: see the kernel's entry) */
+#define SLX_ERR_PAGES (-10)          /* device: not enough free pages or rows */
 
 #define SLX_GEMV_GLU 0
 #define SLX_GEMV_LINEAR 1
@@ -442,6 +443,133 @@ int slx_attn_rope_decode(const void* qkv, int n_q, int n_kv, int head_dim,
                          int max_len, void* k_cache, void* v_cache, void* out,
                          int32_t* status, void* stream);
 int slx_argmax(const void* logits, int T, int V, int32_t* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Batched decode over a paged key-value cache (no reference counterpart: the
+ * reference decodes one request and leaves the cache to mlx-lm).
+ *
+ * The cache of one layer is n_pages pages of page_size tokens,
+ *   pages [n_pages][2 (K, V)][n_kv][page_size][head_dim],
+ * one kv head's page being one contiguous block.  A request's tokens lie in
+ * the pages its block-table row lists, token p in entry p / page_size at
+ * offset p % page_size; token p's slot is page * page_size + p % page_size.
+ * The table and the slots are the same for every layer.
+ *
+ * Rows: a step computes T rows, each one new token of a request (one per
+ * request in plain decode, several for a request whose prompt is fed).  A
+ * padding row has pos = -1 (and req = slot = -1).
+ *
+ * An index outside its range (a page, a request, a slot) sets
+ * SLX_ERR_OUT_OF_RANGE in *status and is never followed. */
+#define SLX_KV_BF16 0
+#define SLX_KV_E4M3 1 /* value = e4m3 * scale of its kv head */
+
+typedef struct slx_kv_pages {
+  void* base;           /* 16-byte aligned */
+  const float* k_scale; /* [n_kv], e4m3 only (NULL for bf16) */
+  const float* v_scale; /* [n_kv] */
+  int32_t n_pages;      /* n_pages * page_size < 2^31 */
+  int32_t page_size;    /* 16, 32, 64, 128 or 256 */
+  int32_t n_kv;
+  int32_t head_dim;     /* 64 or 128 */
+  int32_t dtype;        /* SLX_KV_BF16 or SLX_KV_E4M3 */
+} slx_kv_pages;
+
+/* Plan of one step over n_req requests (at most 8192): hands out pages and
+ * lists the step's rows.
+ *   n_new   [n_req] new tokens of each request (0 = idle, -1 = the request
+ *           is finished: its pages go back to the free stack)
+ *   lengths [n_req] tokens held before the step; lengths_out (may alias):
+ *           after it (0 for a finished request)
+ *   table   [n_req][max_pages] block table, entries of new pages written
+ *   free_list [n_pages] stack of free pages, the first *n_free entries
+ *           valid; n_free_out (may alias n_free): entries left
+ *   row_req, row_pos, row_slot [n_rows]: the rows in request order, then
+ *           padding (-1);  row_start [n_req + 1]: first row of each request
+ * Released pages are pushed in request and table order, then new ones are
+ * popped in that order, so the result does not depend on timing.  Without
+ * the aliases the call may be repeated with the same result.
+ * All or nothing: when the free pages or n_rows do not suffice
+ * (SLX_ERR_PAGES) or an input is out of range (SLX_ERR_OUT_OF_RANGE: n_new <
+ * -1, a length outside 0..max_pages * page_size, *n_free outside 0..n_pages,
+ * more pages than n_pages) the table and the free list stay as they are,
+ * lengths_out = lengths, n_free_out = *n_free, and every row is padding. */
+int slx_paged_plan(const int32_t* n_new, const int32_t* lengths,
+                   int32_t* lengths_out, int n_req, int32_t* table,
+                   int max_pages, int page_size, int32_t* free_list,
+                   int n_pages, const int32_t* n_free, int32_t* n_free_out,
+                   int32_t* row_req, int32_t* row_pos, int32_t* row_slot,
+                   int n_rows, int32_t* row_start, int32_t* status,
+                   void* stream);
+
+/* q/k RMSNorm + rotate-half RoPE + append to the pages, T rows (the paged
+ * form of slx_qk_norm_rope_cache).  qkv [T][qkv_stride]: row t holds n_q,
+ * n_kv and n_kv heads of head_dim bf16; q_out [T][n_q * head_dim] gets the
+ * rotated queries, the pages' slot[t] the rotated key and the value.  The
+ * angle pos * inv_freq is formed in 64 bits; everything else is fp32 and
+ * rounded once.  E4m3 pages: x / scale, to nearest, saturating at 448.
+ * A row with slot < 0 or pos < 0 writes zero queries and no page.  Slots of
+ * one call are distinct. */
+int slx_paged_append(const void* qkv, int64_t qkv_stride, int T, int n_q,
+                     const void* q_norm, const void* k_norm, float eps,
+                     const float* inv_freq, const int32_t* pos,
+                     const int32_t* slot, const slx_kv_pages* pages,
+                     void* q_out, int32_t* status, void* stream);
+
+/* Bytes of workspace slx_paged_attn_decode needs for T rows on the current
+ * device.  Zero before the first call; every call leaves it reusable.  Calls
+ * that may overlap (two streams, two graphs) need workspaces of their own. */
+size_t slx_paged_attn_workspace_bytes(int T, int n_q, int n_kv, int head_dim);
+
+/* Attention of T rows over the pages (GQA, n_q / n_kv <= 16): row t attends
+ * positions 0..pos[t] of request req[t] (req NULL: request t).
+ * q [T][q_stride] bf16 (n_q heads of head_dim), out [T][n_q * head_dim]
+ * bf16.  A row with pos < 0 gives zeros; a row with req or pos out of range
+ * sets *status and gives zeros; keys on a page out of range set *status and
+ * count as absent. */
+int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
+                          const slx_kv_pages* pages, const int32_t* table,
+                          int n_req, int max_pages, const int32_t* req,
+                          const int32_t* pos, float scale, void* out,
+                          void* workspace, size_t workspace_bytes,
+                          int32_t* status, void* stream);
+
+/* What is applied to a step's logits; every pointer may be NULL. */
+typedef struct slx_logit_rules {
+  const int32_t* history;    /* [T][history_stride] the row's token ids:
+                                prompt, then output */
+  const int32_t* n_prompt;   /* [T] prompt tokens of history (NULL: 0) */
+  const int32_t* n_history;  /* [T] tokens of history, prompt included */
+  const float* repetition;   /* [T] divisor of positive, factor of other
+                                logits of every id in the history */
+  const float* frequency;    /* [T] subtracted per occurrence in the output */
+  const float* presence;     /* [T] subtracted once when in the output */
+  const int32_t* bias_ids;   /* [n_bias] ids of all rows' biases ... */
+  const float* bias_values;  /* [n_bias] ... and what is added to them */
+  const int32_t* bias_start; /* [T + 1] row t's entries: start[t]..start[t+1];
+                                at most 8191 a row, an id listed twice takes
+                                its last entry */
+  const uint32_t* mask;      /* [T][mask_stride] bit i of word w allows id
+                                32 w + i; others become -inf */
+  int32_t history_stride;    /* <= 262143 */
+  int32_t n_bias;
+  int32_t mask_stride;       /* >= ceil(V / 32) */
+} slx_logit_rules;
+
+/* Penalties, biases and grammar mask on the logits of T rows, and the greedy
+ * pick, in one launch (slx_argmax with the rules applied first).
+ *   logits [T][V] bf16 (f32 = 0) or fp32 (f32 = 1)
+ *   out    [T][V] of the same type, or NULL; may be logits itself
+ *   pick   [T] lowest id among the greatest allowed logits, or NULL; -1
+ *          when the mask allows none.  A NaN logit counts as -inf here.
+ * In order: repetition, frequency, presence, bias, mask.  Ids the rules
+ * touch are computed in fp64 and picked by that value; out is rounded once.
+ * History ids outside 0..V-1 are ignored, bias ids outside it too; counts or
+ * bias ranges outside their arrays set SLX_ERR_OUT_OF_RANGE in *status and
+ * are clipped. */
+int slx_logits_process(const void* logits, int f32, int T, int V,
+                       const slx_logit_rules* rules, void* out, int32_t* pick,
+                       int32_t* status, void* stream);
 
 /* Read n byte ranges of files: fds[i] from offsets[i], sizes[i] bytes,
  * into dsts[i], on up to `threads` native threads (a pool shared by all

@@ -21,9 +21,11 @@ ERRORS = {
     -1: "SLX_ERR_INVALID", -2: "SLX_ERR_UNSUPPORTED", -3: "SLX_ERR_CUDA",
     -4: "SLX_ERR_OUT_OF_RANGE", -5: "SLX_ERR_UNMAPPED_EXPERT",
     -6: "SLX_ERR_DEVICE_TIMEOUT", -7: "SLX_ERR_SCRATCH", -8: "SLX_ERR_IO",
-    -9: "SLX_ERR_RANGE",
+    -9: "SLX_ERR_RANGE", -10: "SLX_ERR_PAGES",
 }
+SLX_ERR_OUT_OF_RANGE = -4
 SLX_ERR_RANGE = -9
+SLX_ERR_PAGES = -10
 GEMV_GLU, GEMV_LINEAR = 0, 1
 
 # every symbol the header declares (the CPU test checks they are exported)
@@ -44,6 +46,8 @@ EXPORTS = (
     "slx_switchglu_serviced", "slx_host_device_ptr",
     "slx_ep_grid", "slx_switchglu_ep", "slx_ep_combine_rmsnorm",
     "slx_ipc_handle", "slx_ipc_open", "slx_ipc_close",
+    "slx_paged_plan", "slx_paged_append", "slx_paged_attn_workspace_bytes",
+    "slx_paged_attn_decode", "slx_logits_process",
 )
 EP_MAX_RANKS = 8
 
@@ -67,6 +71,26 @@ class slx_expert_bank(C.Structure):
 
 class slx_shared_expert(C.Structure):
     _fields_ = [("base", C.c_void_p), ("inter", C.c_int32)]
+
+
+KV_BF16, KV_E4M3 = 0, 1
+
+
+class slx_kv_pages(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class slx_logit_rules(C.Structure):
+    _fields_ = [("history", C.c_void_p), ("n_prompt", C.c_void_p),
+                ("n_history", C.c_void_p), ("repetition", C.c_void_p),
+                ("frequency", C.c_void_p), ("presence", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
+                ("bias_start", C.c_void_p), ("mask", C.c_void_p),
+                ("history_stride", C.c_int32), ("n_bias", C.c_int32),
+                ("mask_stride", C.c_int32)]
 
 
 class SlxError(RuntimeError):
@@ -221,6 +245,24 @@ def lib() -> C.CDLL:
         L.slx_prefill_grouped.argtypes = [C.POINTER(slx_expert_bank), vp, i32,
                                           vp, i32, vp, i32, vp, vp, i32, vp,
                                           sz, vp, vp]
+        L.slx_paged_plan.restype = i32
+        L.slx_paged_plan.argtypes = [vp, vp, vp, i32, vp, i32, i32, vp, i32,
+                                     vp, vp, vp, vp, vp, i32, vp, vp, vp]
+        L.slx_paged_append.restype = i32
+        L.slx_paged_append.argtypes = [vp, C.c_int64, i32, i32, vp, vp,
+                                       C.c_float, vp, vp, vp,
+                                       C.POINTER(slx_kv_pages), vp, vp, vp]
+        L.slx_paged_attn_workspace_bytes.restype = sz
+        L.slx_paged_attn_workspace_bytes.argtypes = [i32, i32, i32, i32]
+        L.slx_paged_attn_decode.restype = i32
+        L.slx_paged_attn_decode.argtypes = [vp, C.c_int64, i32, i32,
+                                            C.POINTER(slx_kv_pages), vp, i32,
+                                            i32, vp, vp, C.c_float, vp, vp,
+                                            sz, vp, vp]
+        L.slx_logits_process.restype = i32
+        L.slx_logits_process.argtypes = [vp, i32, i32, i32,
+                                         C.POINTER(slx_logit_rules), vp, vp,
+                                         vp, vp]
         _lib = L
     return _lib
 
@@ -568,6 +610,76 @@ def argmax(logits, out, stream=None) -> None:
     rc = lib().slx_argmax(logits.data_ptr(), T, V, out.data_ptr(),
                           stream_ptr(stream))
     _check("slx_argmax", rc)
+    _count(1)
+
+
+def paged_plan(n_new, lengths, lengths_out, table, page_size: int, free_list,
+               n_free, n_free_out, row_req, row_pos, row_slot, row_start,
+               status, stream: int) -> None:
+    """Pages and rows of one step over the requests (stream: raw handle)."""
+    rc = lib().slx_paged_plan(
+        n_new.data_ptr(), lengths.data_ptr(), lengths_out.data_ptr(),
+        table.shape[0], table.data_ptr(), table.shape[1], page_size,
+        free_list.data_ptr(), free_list.shape[0], n_free.data_ptr(),
+        n_free_out.data_ptr(), row_req.data_ptr(), row_pos.data_ptr(),
+        row_slot.data_ptr(), row_req.shape[0], row_start.data_ptr(),
+        status.data_ptr(), stream)
+    _check("slx_paged_plan", rc)
+    _count(1)
+
+
+def kv_pages(pages: torch.Tensor, kv_scale) -> slx_kv_pages:
+    """pages [n_pages, 2, n_kv, page_size, head_dim]; kv_scale [2, n_kv]
+    fp32 (e4m3 pages) or None."""
+    n, _, n_kv, ps, hd = pages.shape
+    if kv_scale is None:
+        return slx_kv_pages(pages.data_ptr(), None, None, n, ps, n_kv, hd,
+                            KV_BF16)
+    k = kv_scale.data_ptr()
+    return slx_kv_pages(pages.data_ptr(), k, k + 4 * n_kv, n, ps, n_kv, hd,
+                        KV_E4M3)
+
+
+def paged_append(qkv, pages: slx_kv_pages, slot, pos, n_q: int, q_norm,
+                 k_norm, eps: float, inv_freq, q_out, status,
+                 stream: int) -> None:
+    """q/k norm + RoPE, queries to q_out, keys and values to the pages."""
+    rc = lib().slx_paged_append(
+        qkv.data_ptr(), qkv.stride(0), qkv.shape[0], n_q, q_norm.data_ptr(),
+        k_norm.data_ptr(), eps, inv_freq.data_ptr(), pos.data_ptr(),
+        slot.data_ptr(), C.byref(pages), q_out.data_ptr(), status.data_ptr(),
+        stream)
+    _check("slx_paged_append", rc)
+    _count(1)
+
+
+def paged_attn_workspace_bytes(T: int, n_q: int, n_kv: int,
+                               head_dim: int) -> int:
+    return int(lib().slx_paged_attn_workspace_bytes(T, n_q, n_kv, head_dim))
+
+
+def paged_attn_decode(q, q_stride: int, n_q: int, pages: slx_kv_pages, table,
+                      req, pos, scale: float, out, workspace, status,
+                      stream: int) -> None:
+    """Attention of pos.shape[0] rows over the pages."""
+    rc = lib().slx_paged_attn_decode(
+        q.data_ptr(), q_stride, pos.shape[0], n_q, C.byref(pages),
+        table.data_ptr(), table.shape[0], table.shape[1], ptr(req),
+        pos.data_ptr(), scale, out.data_ptr(), ptr(workspace),
+        0 if workspace is None else workspace.shape[0], status.data_ptr(),
+        stream)
+    _check("slx_paged_attn_decode", rc)
+    _count(1)
+
+
+def logits_process(logits, rules: slx_logit_rules, out, pick, status,
+                   stream: int) -> None:
+    """Penalties, biases, mask and greedy pick of logits [T, V]."""
+    rc = lib().slx_logits_process(
+        logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0,
+        logits.shape[0], logits.shape[1], C.byref(rules), ptr(out), ptr(pick),
+        status.data_ptr(), stream)
+    _check("slx_logits_process", rc)
     _count(1)
 
 

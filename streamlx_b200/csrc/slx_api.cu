@@ -805,6 +805,179 @@ int slx_argmax(const void* logits, int T, int V, int32_t* out, void* stream) {
   return rc ? cuda_check(rc, "slx_argmax") : SLX_OK;
 }
 
+namespace {
+
+int pages_ok(const slx_kv_pages* p, const char* what, slx::KvPages* out) {
+  if (!p || !p->base || !aligned16(p->base))
+    return fail(SLX_ERR_INVALID, "%s: pages NULL or not 16-byte aligned", what);
+  if (p->dtype != SLX_KV_BF16 && p->dtype != SLX_KV_E4M3)
+    return fail(SLX_ERR_UNSUPPORTED, "%s: page dtype %d", what, p->dtype);
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return fail(SLX_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, p->head_dim);
+  const int ps = p->page_size;
+  if (ps < 16 || ps > 256 || (ps & (ps - 1)))
+    return fail(SLX_ERR_UNSUPPORTED, "%s: page_size %d (16, 32, 64, 128, 256)", what, ps);
+  if (p->n_pages < 1 || (long long)p->n_pages * ps > 0x7fffffffLL || p->n_kv < 1)
+    return fail(SLX_ERR_INVALID, "%s: n_pages %d n_kv %d", what, p->n_pages, p->n_kv);
+  if (p->dtype == SLX_KV_E4M3 && (!p->k_scale || !p->v_scale))
+    return fail(SLX_ERR_INVALID, "%s: e4m3 pages need k_scale and v_scale", what);
+  if (p->dtype == SLX_KV_BF16 && (p->k_scale || p->v_scale))
+    return fail(SLX_ERR_INVALID, "%s: bf16 pages take no scales", what);
+  *out = {reinterpret_cast<uint8_t*>(p->base), p->k_scale, p->v_scale,
+          p->n_pages, ps, p->n_kv, p->head_dim};
+  return SLX_OK;
+}
+
+}  // namespace
+
+int slx_paged_plan(const int32_t* n_new, const int32_t* lengths,
+                   int32_t* lengths_out, int n_req, int32_t* table,
+                   int max_pages, int page_size, int32_t* free_list,
+                   int n_pages, const int32_t* n_free, int32_t* n_free_out,
+                   int32_t* row_req, int32_t* row_pos, int32_t* row_slot,
+                   int n_rows, int32_t* row_start, int32_t* status,
+                   void* stream) {
+  g_err.clear();
+  if (!n_new || !lengths || !lengths_out || !table || !free_list || !n_free ||
+      !n_free_out || !row_start)
+    return fail(SLX_ERR_INVALID, "paged_plan: NULL pointer");
+  if (n_rows < 0 || (n_rows > 0 && (!row_req || !row_pos || !row_slot)))
+    return fail(SLX_ERR_INVALID, "paged_plan: n_rows %d", n_rows);
+  if (n_req < 1 || n_req > 8192)
+    return fail(SLX_ERR_UNSUPPORTED, "paged_plan: n_req %d (1..8192)", n_req);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(SLX_ERR_UNSUPPORTED, "paged_plan: page_size %d", page_size);
+  if (max_pages < 1 || n_pages < 1 ||
+      (long long)max_pages * page_size > 0x7fffffffLL ||
+      (long long)n_pages * page_size > 0x7fffffffLL)
+    return fail(SLX_ERR_INVALID, "paged_plan: max_pages %d n_pages %d", max_pages, n_pages);
+  const slx::PlanArgs a = {n_new, lengths, lengths_out, n_req, table, max_pages,
+                           page_size, free_list, n_pages, n_free, n_free_out,
+                           row_req, row_pos, row_slot, n_rows, row_start, status};
+  const int rc = slx::launch_paged_plan(a, reinterpret_cast<cudaStream_t>(stream));
+  return rc ? cuda_check(rc, "slx_paged_plan") : SLX_OK;
+}
+
+int slx_paged_append(const void* qkv, int64_t qkv_stride, int T, int n_q,
+                     const void* q_norm, const void* k_norm, float eps,
+                     const float* inv_freq, const int32_t* pos,
+                     const int32_t* slot, const slx_kv_pages* pages,
+                     void* q_out, int32_t* status, void* stream) {
+  g_err.clear();
+  slx::AppendArgs a = {};
+  const int bad = pages_ok(pages, "paged_append", &a.kv);
+  if (bad) return bad;
+  if (T < 0 || n_q < 1 || n_q % a.kv.n_kv || n_q + 2 * (long long)a.kv.n_kv > 65535)
+    return fail(SLX_ERR_INVALID, "paged_append: T %d n_q %d n_kv %d", T, n_q, a.kv.n_kv);
+  if (T == 0) return SLX_OK;
+  if (!qkv || !q_norm || !k_norm || !inv_freq || !pos || !slot || !q_out)
+    return fail(SLX_ERR_INVALID, "paged_append: NULL pointer");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm))
+    return fail(SLX_ERR_INVALID, "paged_append: qkv / q_out / norms not 16-byte aligned");
+  if (qkv_stride % 8 || qkv_stride < (int64_t)(n_q + 2 * a.kv.n_kv) * a.kv.hd)
+    return fail(SLX_ERR_INVALID, "paged_append: qkv_stride %lld", (long long)qkv_stride);
+  a.qkv = (const uint16_t*)qkv;
+  a.stride = qkv_stride;
+  a.T = T;
+  a.nq = n_q;
+  a.qn = (const uint16_t*)q_norm;
+  a.kn = (const uint16_t*)k_norm;
+  a.eps = eps;
+  a.inv_freq = inv_freq;
+  a.pos = pos;
+  a.slot = slot;
+  a.q_out = (uint16_t*)q_out;
+  a.status = status;
+  const int rc = slx::launch_paged_append(a, pages->dtype == SLX_KV_E4M3,
+                                          reinterpret_cast<cudaStream_t>(stream));
+  return rc ? cuda_check(rc, "slx_paged_append") : SLX_OK;
+}
+
+size_t slx_paged_attn_workspace_bytes(int T, int n_q, int n_kv, int head_dim) {
+  if (T < 0 || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q / n_kv > 16 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return slx::paged_attn_workspace_bytes(T, n_q, n_kv, head_dim);
+}
+
+int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
+                          const slx_kv_pages* pages, const int32_t* table,
+                          int n_req, int max_pages, const int32_t* req,
+                          const int32_t* pos, float scale, void* out,
+                          void* workspace, size_t workspace_bytes,
+                          int32_t* status, void* stream) {
+  g_err.clear();
+  slx::PagedAttnArgs a = {};
+  const int bad = pages_ok(pages, "paged_attn", &a.kv);
+  if (bad) return bad;
+  if (T < 0 || n_q < 1 || n_q % a.kv.n_kv || n_q / a.kv.n_kv > 16)
+    return fail(SLX_ERR_INVALID, "paged_attn: T %d n_q %d n_kv %d (at most 16 q heads a kv head)",
+                T, n_q, a.kv.n_kv);
+  if (n_req < 1 || max_pages < 1 || (long long)max_pages * a.kv.page_size > 0x7fffffffLL)
+    return fail(SLX_ERR_INVALID, "paged_attn: n_req %d max_pages %d", n_req, max_pages);
+  if (!req && T > n_req)
+    return fail(SLX_ERR_INVALID, "paged_attn: T %d rows, %d requests and no req", T, n_req);
+  if (T == 0) return SLX_OK;
+  if (!q || !table || !pos || !out)
+    return fail(SLX_ERR_INVALID, "paged_attn: NULL pointer");
+  if (!aligned16(q) || !aligned16(out) || q_stride % 8 ||
+      q_stride < (int64_t)n_q * a.kv.hd)
+    return fail(SLX_ERR_INVALID, "paged_attn: q / out alignment or q_stride %lld", (long long)q_stride);
+  const size_t need = slx::paged_attn_workspace_bytes(T, n_q, a.kv.n_kv, a.kv.hd);
+  if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(SLX_ERR_SCRATCH, "paged_attn: workspace %zu < %zu bytes (or not 16-byte aligned)",
+                workspace ? workspace_bytes : (size_t)0, need);
+  a.q = (const uint16_t*)q;
+  a.q_stride = q_stride;
+  a.T = T;
+  a.nq = n_q;
+  a.table = table;
+  a.n_req = n_req;
+  a.max_pages = max_pages;
+  a.req = req;
+  a.pos = pos;
+  a.scale = scale;
+  a.out = (uint16_t*)out;
+  a.ws = workspace;
+  a.status = status;
+  const int rc = slx::launch_paged_attn(a, pages->dtype == SLX_KV_E4M3,
+                                        reinterpret_cast<cudaStream_t>(stream));
+  return rc ? cuda_check(rc, "slx_paged_attn_decode") : SLX_OK;
+}
+
+int slx_logits_process(const void* logits, int f32, int T, int V,
+                       const slx_logit_rules* rules, void* out, int32_t* pick,
+                       int32_t* status, void* stream) {
+  g_err.clear();
+  slx::LogitArgs a = {};
+  if (T < 0 || V < 1) return fail(SLX_ERR_INVALID, "logits: T %d V %d", T, V);
+  if (T == 0) return SLX_OK;
+  if (!logits || (!out && !pick))
+    return fail(SLX_ERR_INVALID, "logits: NULL logits, or neither out nor pick");
+  const uintptr_t el = f32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & el)
+    return fail(SLX_ERR_INVALID, "logits: misaligned");
+  if (rules) a.r = *rules;
+  if (a.r.history && (!a.r.n_history || a.r.history_stride < 0 || a.r.history_stride > 262143))
+    return fail(SLX_ERR_INVALID, "logits: history needs n_history and a stride of at most 262143, got %d",
+                a.r.history_stride);
+  if (!a.r.history && (a.r.repetition || a.r.frequency || a.r.presence))
+    return fail(SLX_ERR_INVALID, "logits: penalties need a history");
+  if (!!a.r.bias_ids != !!a.r.bias_values || !!a.r.bias_ids != !!a.r.bias_start ||
+      (a.r.bias_ids && a.r.n_bias < 0))
+    return fail(SLX_ERR_INVALID, "logits: bias_ids, bias_values and bias_start belong together");
+  if (a.r.mask && a.r.mask_stride < (V - 1) / 32 + 1)
+    return fail(SLX_ERR_INVALID, "logits: mask_stride %d for V %d", a.r.mask_stride, V);
+  a.logits = logits;
+  a.T = T;
+  a.V = V;
+  a.out = out;
+  a.pick = pick;
+  a.status = status;
+  const int rc = slx::launch_logits(a, f32 != 0, reinterpret_cast<cudaStream_t>(stream));
+  return rc ? cuda_check(rc, "slx_logits_process") : SLX_OK;
+}
+
 int slx_copy_many(void* const* dst, const void* const* src,
                   const size_t* bytes, int n, void* stream) {
   g_err.clear();

@@ -136,6 +136,72 @@ int launch_attn_rope_decode(const uint16_t* qkv, int nq, int nkv, int hd,
                             uint16_t* out, int32_t* status, cudaStream_t s);
 int launch_argmax(const uint16_t* logits, int T, int V, int32_t* out,
                   cudaStream_t s);
+// One layer's paged KV cache as the kernels see it (slx_kv_pages).
+struct KvPages {
+  uint8_t* base;
+  const float* k_scale;
+  const float* v_scale;
+  int n_pages, page_size, n_kv, hd;
+};
+
+struct PlanArgs {
+  const int32_t* n_new;
+  const int32_t* lengths;
+  int32_t* lengths_out;
+  int n_req;
+  int32_t* table;
+  int max_pages, page_size;
+  int32_t* free_list;
+  int n_pages;
+  const int32_t* n_free;
+  int32_t* n_free_out;
+  int32_t *row_req, *row_pos, *row_slot;
+  int n_rows;
+  int32_t* row_start;
+  int32_t* status;
+};
+
+struct AppendArgs {
+  const uint16_t* qkv;
+  long long stride;
+  int T, nq;
+  const uint16_t *qn, *kn;
+  float eps;
+  const float* inv_freq;
+  const int32_t *pos, *slot;
+  KvPages kv;
+  uint16_t* q_out;
+  int32_t* status;
+};
+
+struct PagedAttnArgs {
+  const uint16_t* q;
+  long long q_stride;
+  int T, nq;
+  KvPages kv;
+  const int32_t* table;
+  int n_req, max_pages;
+  const int32_t *req, *pos;
+  float scale;
+  uint16_t* out;
+  void* ws;
+  int32_t* status;
+};
+
+struct LogitArgs {
+  const void* logits;
+  int T, V;
+  slx_logit_rules r;
+  void* out;
+  int32_t* pick;
+  int32_t* status;
+};
+
+int launch_paged_plan(const PlanArgs& a, cudaStream_t s);
+int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s);
+size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd);
+int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s);
+int launch_logits(const LogitArgs& a, bool f32, cudaStream_t s);
 size_t prefill_scratch_bytes(int n_blocks, int H, int I);
 int launch_prefill(const uint8_t* bank, long long slot_stride, int n_slots,
                    int H, int I, const uint16_t* x, int n_rows,

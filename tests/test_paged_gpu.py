@@ -1,0 +1,564 @@
+"""Batched decode over a paged KV cache against plain 64-bit restatements
+(tests/paged_cases.py): the step's plan, the append and the attention."""
+
+import numpy as np
+import pytest
+import torch
+
+from streamlx_b200 import _lib as L
+from streamlx_b200 import ops
+from tests import paged_cases as P
+
+pytestmark = pytest.mark.gpu
+
+BF, E4 = torch.bfloat16, torch.float8_e4m3fn
+EPS = 1e-6
+
+
+def dev_cache(*args, **kw):
+    pages, sc, table = P.make_cache(*args, **kw)
+    return (pages, sc, table), (pages.cuda(), None if sc is None else sc.cuda(),
+                                table.cuda())
+
+
+def queries(T, nq, hd, seed=1, std=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, nq, hd, generator=g) * std).to(BF)
+
+
+def run_attention(q, dev, req, pos, scale=None, **kw):
+    pages, sc, table = dev
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = ops.paged_attention(
+        q.cuda(), pages, table, torch.tensor(pos, dtype=torch.int32).cuda(),
+        req=None if req is None else torch.tensor(req, dtype=torch.int32).cuda(),
+        scale=scale, kv_scale=sc, status=st, **kw)
+    torch.cuda.synchronize()
+    return out.cpu(), int(st.item())
+
+
+def check_attention(q, host, dev, req, pos, scale=None, **kw):
+    page, hd = host[0].shape[3], host[0].shape[4]
+    out, st = run_attention(q, dev, req, pos, scale, **kw)
+    assert st == 0
+    want, bound = P.attention(q, host[0], host[1], host[2],
+                              req or range(len(pos)), pos, page,
+                              hd ** -0.5 if scale is None else scale)
+    err = (out.double() - want).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= bound).all(), float((err / bound.clamp(min=1e-30)).max())
+    return out
+
+
+# ------------------------------------------------------------- attention --
+
+HEADS = [(24, 4), (16, 2), (1, 1), (8, 8), (32, 2), (9, 3), (12, 1)]
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,nkv", HEADS)
+def test_attention_ragged(nq, nkv, hd, dtype):
+    """Lengths around page and tile ends, an idle row, NaN in every place of
+    the cache that no row holds, -1 in the table behind the last page."""
+    lens = [1, 0, 15, 16, 17, 33, 64, 100, 129, 255]
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=nq + hd)
+    q = queries(len(lens), nq, hd)
+    out = check_attention(q, host, dev, None, [n - 1 for n in lens])
+    assert (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_attention_pages(page, dtype):
+    lens = [page - 1, page, page + 1, 3 * page + 5, 700]
+    host, dev = dev_cache(lens, 2, 128, page, dtype, seed=page)
+    check_attention(queries(len(lens), 16, 128), host, dev, None,
+                    [n - 1 for n in lens])
+
+
+@pytest.mark.parametrize("nq,nkv,hd,dtype,lens", [
+    (16, 2, 128, BF, [20000]), (24, 4, 128, E4, [9001, 3, 0, 1]),
+    (8, 1, 64, BF, [1, 12345, 2]), (4, 4, 64, E4, [8192])])
+def test_attention_long(nq, nkv, hd, dtype, lens):
+    """The cache's length split over many CTAs and joined."""
+    host, dev = dev_cache(lens, nkv, hd, 32, dtype, seed=3)
+    check_attention(queries(len(lens), nq, hd), host, dev, None,
+                    [n - 1 for n in lens])
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_many_rows(dtype):
+    """More rows than CTAs of one wave, short and long ones mixed."""
+    g = np.random.default_rng(5)
+    lens = [int(n) for n in g.integers(0, 60, 600)]
+    lens[17], lens[599] = 3000, 900
+    host, dev = dev_cache(lens, 2, 64, 16, dtype, seed=9)
+    check_attention(queries(len(lens), 4, 64), host, dev, None,
+                    [n - 1 for n in lens])
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_prompt_rows(dtype):
+    """Several rows of one request (each its own causal length), requests in
+    any order, padding rows, the same row twice."""
+    lens = [70, 5, 300]
+    host, dev = dev_cache(lens, 4, 128, 16, dtype, seed=4)
+    req = [2] * 20 + [0] * 9 + [-1] + [1] + [0] + [2, 2]
+    pos = [280 + i for i in range(20)] + [61 + i for i in range(9)] + \
+        [-1] + [4] + [0] + [31, 31]
+    out = check_attention(queries(len(req), 24, 128), host, dev, req, pos)
+    assert (out[29] == 0).all()
+
+
+def test_attention_strided_queries():
+    """q as the head part of wider rows, and a row stride beyond them."""
+    lens = [40, 7, 90]
+    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=6)
+    wide = torch.randn(3, 24 * 128 + 64).to(BF).cuda()
+    q = wide[:, 128:128 + 16 * 128].unflatten(1, (16, 128))
+    pages, sc, table = dev
+    pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32).cuda()
+    a = ops.paged_attention(q, pages, table, pos)
+    b = ops.paged_attention(q.contiguous(), pages, table, pos)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scale", [0.0, 40.0, -1.0])
+def test_attention_extreme_scores(scale):
+    """Equal scores, scores far apart (one key takes all), a negative scale."""
+    lens = [500, 3, 64]
+    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=7)
+    check_attention(queries(3, 16, 128), host, dev, None,
+                    [n - 1 for n in lens], scale=scale)
+
+
+def test_attention_infinite_and_nan_keys():
+    """What the rows do hold follows the formula: an infinite score takes a
+    row's weight away or makes it NaN, and touches no other row."""
+    lens = [30, 200, 31]
+    host, dev = dev_cache(lens, 1, 64, 16, BF, seed=8)
+    pages, _, table = dev
+    q = torch.ones(3, 2, 64, dtype=BF)
+    page0, page2 = int(host[2][0, 1]), int(host[2][2, 0])
+    pages[page0, 0, 0, 3] = float("-inf")         # request 0, key 19: weight 0
+    pages[page2, 0, 0, 5] = float("nan")          # request 2: NaN
+    out, st = run_attention(q, dev, None, [29, 199, 30])
+    assert st == 0 and torch.isnan(out[2]).all()
+    h = host[0].clone()
+    h[page0, 0, 0, 3] = float("-inf")
+    want, _ = P.attention(q, h, None, host[2], [0, 1, 2], [29, 199, -1], 16,
+                          64 ** -0.5)
+    err = (out[:2].double() - want[:2]).abs()
+    assert (err <= 2.0 ** -7 * want[:2].abs() + 1e-3).all()
+    # every key of a row at -inf: nothing to divide by, NaN as the formula
+    pages[int(host[2][0, 0]), 0] = float("-inf")
+    pages[page0, 0] = float("-inf")
+    out, st = run_attention(q, dev, None, [29, 199, -1])
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
+
+
+def test_attention_bad_indices():
+    """A page, request or position out of range sets the status, is not
+    followed, and leaves the other rows right."""
+    lens = [40, 50, 60]
+    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=10)
+    pages, sc, table = dev
+    q = queries(3, 16, 128)
+    good = check_attention(q, host, dev, None, [39, 49, 59])
+    for bad in (-1, pages.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[1, 2] = bad
+        out, st = run_attention(q, (pages, sc, t), None, [39, 49, 59])
+        assert st == L.SLX_ERR_OUT_OF_RANGE
+        assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+    cap = table.shape[1] * 16
+    for req, pos in (([0, 3, 2], [39, 49, 59]), ([0, -1, 2], [39, 49, 59]),
+                     ([0, 1, 2], [39, cap, 59]),
+                     ([0, 1, 2], [39, 2 ** 31 - 1, 59])):
+        out, st = run_attention(q, dev, req, pos)
+        assert st == L.SLX_ERR_OUT_OF_RANGE
+        assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+        assert (out[1] == 0).all()
+
+
+def test_attention_same_bits_again():
+    """Repeated calls on one workspace give the same bits: the joins do not
+    depend on which CTA comes last."""
+    lens = [5000, 40, 0, 2500, 1]
+    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=11)
+    q, pos = queries(5, 16, 128), [n - 1 for n in lens]
+    ws = ops.paged_workspace(5, 16, 2, 128, "cuda")
+    first, _ = run_attention(q, dev, None, pos, workspace=ws)
+    for _ in range(20):
+        out, st = run_attention(q, dev, None, pos, workspace=ws)
+        assert st == 0 and torch.equal(out, first)
+
+
+def test_attention_streams_and_graphs():
+    """Calls on two streams at once, and two captured graphs replayed side by
+    side with changed lengths, each as the call alone."""
+    lens = [3000, 77, 1500]
+    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=12)
+    pages, sc, table = dev
+    q = [queries(3, 16, 128, seed=s).cuda() for s in (1, 2)]
+    pos = [torch.tensor(p, dtype=torch.int32).cuda()
+           for p in ([2999, 76, 1499], [1200, -1, 900])]
+    want = [[ops.paged_attention(q[i], pages, table, pos[j]).clone()
+             for j in range(2)] for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        outs = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs.append(ops.paged_attention(q[i], pages, table, pos[i]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i][i]) for i in range(2))
+    graphs, outs, live = [], [], [p.clone() for p in pos]
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.paged_attention(q[i], pages, table, live[i]))
+        graphs.append(g)
+    for j in ((0, 1), (1, 0), (1, 1)):
+        for i in range(2):
+            live[i].copy_(pos[j[i]])
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i][j[i]]) for i in range(2))
+
+
+def test_attention_far_pages():
+    """Pages whose element offsets pass 2^32."""
+    n_kv, hd, page = 8, 128, 64
+    per = 2 * n_kv * page * hd
+    n_pages = 2 ** 32 // per + 40
+    pages = torch.empty(n_pages, 2, n_kv, page, hd, dtype=E4, device="cuda")
+    sc = torch.full((2, n_kv), 0.02, device="cuda")
+    ids = [n_pages - 1, 3, n_pages - 7, 2 ** 31 // per + 1]
+    lens = [250, 100]
+    table = torch.full((2, 5), -1, dtype=torch.int32)
+    table[0, :4] = torch.tensor(ids)
+    table[1, :2] = torch.tensor([n_pages - 9, 11])
+    used = [i for i in table.reshape(-1).tolist() if i >= 0]
+    g = torch.Generator().manual_seed(0)
+    small = (torch.randn(len(used), 2, n_kv, page, hd, generator=g) * 50).to(E4)
+    for j, i in enumerate(used):
+        pages[i].copy_(small[j])
+    near = torch.full_like(table, -1)
+    near[0, :4] = torch.arange(4)
+    near[1, :2] = torch.arange(4, 6)
+    q = queries(2, 32, hd)
+    out, st = run_attention(q, (pages, sc, table.cuda()), None, [249, 99])
+    want, bound = P.attention(q, small, sc.cpu(), near, [0, 1], [249, 99],
+                              page, hd ** -0.5)
+    assert st == 0 and ((out.double() - want).abs() <= bound).all()
+
+
+def test_attention_no_rows_and_grid_limit():
+    """No rows; more rows than a grid's second dimension takes."""
+    lens = [20, 33]
+    host, dev = dev_cache(lens, 1, 64, 16, BF, seed=13)
+    pages, sc, table = dev
+    q = queries(0, 2, 64)
+    assert ops.paged_attention(q.cuda(), pages, table, torch.empty(
+        0, dtype=torch.int32, device="cuda")).shape == (0, 2, 64)
+    T = 70001
+    few = queries(2, 2, 64)
+    req = torch.arange(T, dtype=torch.int32).cuda() % 2
+    pos = torch.where(req == 0, 19, 32).to(torch.int32)
+    out = ops.paged_attention(few.cuda()[req.long()].contiguous(), pages,
+                              table, pos, req=req)
+    want = run_attention(few, dev, None, [19, 32])[0].cuda()
+    assert torch.equal(out, want[req.long()])
+
+
+# ---------------------------------------------------------------- append --
+
+def append_case(T, nq, nkv, hd, page, dtype, pos, seed=0, std=2.0):
+    g = torch.Generator().manual_seed(seed)
+    n_pages = T // page + 4
+    pages = (torch.randn(n_pages, 2, nkv, page, hd, generator=g)).to(dtype)
+    sc = None if dtype == BF else torch.rand(2, nkv, generator=g) * .02 + .01
+    slot = torch.randperm(n_pages * page, generator=g)[:T].to(torch.int32)
+    qkv = (torch.randn(T, (nq + 2 * nkv) * hd, generator=g) * std).to(BF)
+    qn, kn = ((1 + .2 * torch.randn(hd, generator=g)).to(BF) for _ in "qk")
+    inv = (1e6 ** (-torch.arange(hd // 2, dtype=torch.float64) / (hd // 2))
+           ).float()
+    return dict(qkv=qkv, pages=pages, sc=sc, slot=slot,
+                pos=torch.tensor(pos, dtype=torch.int32), qn=qn, kn=kn,
+                inv=inv)
+
+
+def run_append(c, nq, **kw):
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    pages = c["pages"].cuda()
+    q = ops.paged_append(
+        c["qkv"].cuda() if "dev_qkv" not in c else c["dev_qkv"], pages,
+        c["slot"].cuda(), c["pos"].cuda(), nq, c["qn"].cuda(), c["kn"].cuda(),
+        EPS, c["inv"].cuda(),
+        kv_scale=None if c["sc"] is None else c["sc"].cuda(), status=st, **kw)
+    return q.cpu(), pages.cpu(), int(st.item())
+
+
+def check_append(c, nq, nkv, hd, page):
+    """q and keys: the 64-bit value rounded once (bf16 2^-8 relative, e4m3
+    2^-4 or half a subnormal step 2^-10), and 2^-18 of the rotated pair's
+    length for the fp32 arithmetic before it (norm, sine and cosine, two
+    products: under 32 steps of 2^-24).  Values: copied, or rounded once."""
+    q, pages, st = run_append(c, nq)
+    assert st == 0
+    T = c["qkv"].shape[0]
+    x = c["qkv"].double().reshape(T, nq + 2 * nkv, hd)
+    y = torch.cat([P.rope(x[:, :nq], c["qn"], c["pos"], c["inv"], EPS),
+                   P.rope(x[:, nq:nq + nkv], c["kn"], c["pos"], c["inv"], EPS),
+                   x[:, nq + nkv:]], 1)
+    pair = (y[..., :hd // 2] ** 2 + y[..., hd // 2:] ** 2).sqrt().repeat(1, 1, 2)
+    slack = 2.0 ** -18 * pair
+    on = (c["slot"] >= 0) & (c["pos"] >= 0)
+    err = (q.double() - y[:, :nq]).abs()
+    assert (err <= 2.0 ** -8 * y[:, :nq].abs() + slack[:, :nq])[on].all()
+    assert (q[~on] == 0).all()
+    want = c["pages"].float().clone()
+    to = c["slot"][on].long()
+    got = pages.float()[to // page, :, :, to % page]     # [T, 2, nkv, hd]
+    kv = torch.stack([y[:, nq:nq + nkv], y[:, nq + nkv:]], 1)[on]
+    sl = torch.stack([slack[:, nq:nq + nkv], 0 * slack[:, nq + nkv:]], 1)[on]
+    if c["sc"] is None:
+        tol = 2.0 ** -8 * kv.abs() + sl
+        assert torch.equal(got[:, 1].double(), kv[:, 1])
+    else:
+        s = c["sc"].double()[None, :, :, None]
+        kv, sl = (kv / s).clamp(-448, 448), sl / s
+        # the quotient's own rounding, 2^-23, stands before the e4m3 one
+        tol = (2.0 ** -4 * kv.abs()).clamp(min=2.0 ** -10) + \
+            2 * sl + 2.0 ** -23 * kv.abs()
+    assert ((got.double() - kv).abs() <= tol).all()
+    # every other place of the pages is as it was, bit for bit
+    want[to // page, :, :, to % page] = got
+    assert torch.equal(pages.float(), want)
+    return q, pages
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,nkv", HEADS)
+def test_append(nq, nkv, hd, dtype):
+    pos = [0, 1, 17, 131071, 5, 1 << 20, 2 ** 31 - 1]
+    c = append_case(len(pos), nq, nkv, hd, 16, dtype, pos, seed=nq)
+    check_append(c, nq, nkv, hd, 16)
+
+
+@pytest.mark.parametrize("T", [1, 2, 333, 5000])
+def test_append_rows(T):
+    pos = [(i * 7919) % 100000 for i in range(T)]
+    c = append_case(T, 16, 2, 128, 64, E4, pos, seed=T)
+    check_append(c, 16, 2, 128, 64)
+
+
+def test_append_padding_and_bad_slots():
+    """Rows without a slot or position: zero queries, no page touched; a slot
+    out of range sets the status and is not written."""
+    c = append_case(6, 8, 2, 128, 16, BF, [3, -1, 5, 9, -1, 7], seed=2)
+    c["slot"][3] = -1
+    check_append(c, 8, 2, 128, 16)
+    c["slot"][5] = c["pages"].shape[0] * 16
+    q, pages, st = run_append(c, 8)
+    assert st == L.SLX_ERR_OUT_OF_RANGE and (q[5] == 0).all()
+    ok = dict(c, slot=c["slot"].clone())
+    ok["slot"][5] = -1
+    q2, pages2, st = run_append(ok, 8)
+    assert st == 0 and torch.equal(q, q2) and torch.equal(pages, pages2)
+
+
+def test_append_saturates_and_zero_rows():
+    """E4m3 values beyond 448 scales saturate, all-zero heads stay zero, NaN
+    stays NaN."""
+    c = append_case(4, 2, 1, 64, 16, E4, [1, 2, 3, 4], seed=3)
+    c["qkv"][0] = 0
+    c["qkv"][1, 3 * 64:] = 3e38
+    c["qkv"][2, 3 * 64:] = -1e30
+    c["qkv"][3, 3 * 64 + 5] = float("nan")
+    q, pages, st = run_append(c, 2)
+    at = [(int(s) // 16, int(s) % 16) for s in c["slot"]]
+    f = pages.float()
+    assert st == 0 and (q[0] == 0).all()
+    assert (f[at[0][0], :, 0, at[0][1]] == 0).all()
+    assert (f[at[1][0], 1, 0, at[1][1]] == 448).all()
+    assert (f[at[2][0], 1, 0, at[2][1]] == -448).all()
+    v = f[at[3][0], 1, 0, at[3][1]]
+    assert torch.isnan(v[5]) and torch.isfinite(v[:5]).all()
+
+
+def test_append_strided_rows():
+    c = append_case(5, 8, 2, 64, 16, BF, [4, 5, 6, 7, 8], seed=4)
+    q, pages, _ = run_append(c, 8)
+    wide = torch.zeros(5, 12 * 64 + 72, dtype=BF, device="cuda")
+    wide[:, :12 * 64] = c["qkv"].cuda()
+    q2, pages2, st = run_append(dict(c, dev_qkv=wide[:, :12 * 64]), 8)
+    assert st == 0 and torch.equal(q, q2) and torch.equal(pages, pages2)
+
+
+# ------------------------------------------------------------------ plan --
+
+class DevicePlan:
+    """Plan state on the device beside its restatement on the host."""
+
+    def __init__(self, n_req, page, n_pages, max_pages, seed=0):
+        self.page, self.ref = page, P.Plan(page, n_pages, max_pages)
+        g = np.random.default_rng(seed)
+        self.lengths = [0] * n_req
+        self.table = [[-1] * max_pages for _ in range(n_req)]
+        self.free = [int(i) for i in g.permutation(n_pages)]
+        self.n_free = n_pages
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.d_len = torch.tensor(self.lengths, **i32)
+        self.d_table = torch.tensor(self.table, **i32)
+        self.d_free = torch.tensor(self.free, **i32)
+        self.d_n = torch.tensor([self.n_free], **i32)
+        self.status = torch.zeros(1, **i32)
+
+    def step(self, n_new, n_rows, alias=True):
+        code, rows, start, self.lengths, self.table, self.free, self.n_free = \
+            self.ref.step(n_new, self.lengths, self.table, self.free,
+                          self.n_free, n_rows)
+        p = ops.paged_plan(
+            torch.tensor(n_new, dtype=torch.int32).cuda(), self.d_len,
+            self.d_table, self.d_free, self.d_n, self.page, n_rows,
+            lengths_out=self.d_len if alias else None,
+            n_free_out=self.d_n if alias else None, status=self.status)
+        self.d_len, self.d_n = p.lengths, p.n_free
+        assert int(self.status.item()) == code
+        self.status.zero_()
+        got = list(zip(p.req.tolist(), p.pos.tolist(), p.slot.tolist()))
+        assert got == rows
+        assert p.start.tolist() == start
+        self.check()
+        return code, p
+
+    def check(self):
+        assert self.d_len.tolist() == self.lengths
+        assert self.d_table.tolist() == self.table
+        assert self.d_free.tolist() == self.free
+        assert self.d_n.tolist() == [self.n_free]
+
+
+@pytest.mark.parametrize("n_req,page,alias", [(1, 16, True), (7, 16, False),
+                                              (65, 32, True), (513, 16, True),
+                                              (8192, 64, True)])
+def test_plan_runs(n_req, page, alias):
+    """Random steps: prompts in chunks, single tokens, idle and finished
+    requests, compared after every step."""
+    max_pages = 9
+    d = DevicePlan(n_req, page, n_req * max_pages // 2 + 5, max_pages)
+    g = np.random.default_rng(n_req)
+    for step in range(12):
+        n_new = []
+        for ln in d.lengths:
+            room = max_pages * page - ln
+            n_new.append(int(g.choice([0, min(1, room), min(1, room),
+                                       int(g.integers(0, min(room, 40) + 1)),
+                                       -1])))
+        d.step(n_new, sum(max(n, 0) for n in n_new) + int(g.integers(0, 70)),
+               alias)
+
+
+def test_plan_large_chunks():
+    """Rows and pages that take several turns of the launch."""
+    d = DevicePlan(40, 16, 20000, 600, seed=3)
+    d.step([9000, 0, 1, 4097] + [16 * i for i in range(36)], 30000)
+    d.step([-1, 5, -1, 1] + [3] * 36, 200)
+
+
+def test_plan_refusals_change_nothing():
+    d = DevicePlan(3, 16, 5, 4)
+    assert d.step([20, 10, 0], 64)[0] == 0
+    assert d.step([10, 10, 10], 29)[0] == L.SLX_ERR_PAGES     # rows
+    assert d.step([1, 40, 16], 64)[0] == L.SLX_ERR_PAGES      # pages
+    assert d.step([1, 55, 0], 64)[0] == L.SLX_ERR_OUT_OF_RANGE  # over the table
+    assert d.step([-2, 0, 0], 64)[0] == L.SLX_ERR_OUT_OF_RANGE
+    assert d.step([2 ** 31 - 1, 0, 0], 64)[0] == L.SLX_ERR_OUT_OF_RANGE
+    assert d.step([2 ** 31 - 1] * 3, 64)[0] == L.SLX_ERR_OUT_OF_RANGE
+    # the pages of a finished request serve the same step
+    assert d.step([-1, 22, 32], 64)[0] == 0
+    d.d_n.fill_(6)
+    d.n_free = 6
+    assert d.step([0, 0, 0], 64)[0] == L.SLX_ERR_OUT_OF_RANGE
+    d.d_n.fill_(0)
+    d.n_free = 0
+    d.d_len[1] = -5
+    d.lengths[1] = -5
+    assert d.step([0, 0, 0], 64)[0] == L.SLX_ERR_OUT_OF_RANGE
+
+
+def test_plan_bad_page_in_table():
+    """A page out of range in the table or on the stack: status, and the row
+    gets no slot."""
+    d = DevicePlan(2, 16, 4, 2)
+    d.step([3, 3], 8)
+    d.d_table[0, 0] = 99
+    p = ops.paged_plan(torch.tensor([1, 1], dtype=torch.int32).cuda(), d.d_len,
+                       d.d_table, d.d_free, d.d_n, 16, 4, status=d.status)
+    assert int(d.status.item()) == L.SLX_ERR_OUT_OF_RANGE
+    assert p.slot.tolist()[0] == -1 and p.slot.tolist()[1] >= 0
+
+
+def test_plan_no_rows_and_repeats():
+    d = DevicePlan(2, 16, 8, 4)
+    d.step([0, 0], 0)
+    d.step([17, 1], 20)
+    args = (torch.tensor([30, -1], dtype=torch.int32).cuda(), d.d_len,
+            d.d_table, d.d_free, d.d_n, 16, 40)
+    a = [t.clone() for t in ops.paged_plan(*args)]
+    table, free = d.d_table.clone(), d.d_free.clone()
+    b = ops.paged_plan(*args)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(table, d.d_table) and torch.equal(free, d.d_free)
+
+
+# -------------------------------------------------------------- together --
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_steps_together(dtype):
+    """Plan, append and attention of several steps as a server runs them:
+    chunks of prompts, single tokens, a finished request whose pages another
+    one takes over; each step's attention against the 64-bit attention over
+    everything the request was given."""
+    nq, nkv, hd, page = 8, 2, 64, 16
+    d = DevicePlan(4, page, 12, 6)
+    pages = torch.full((12, 2, nkv, page, hd), float("nan")).to(dtype).cuda()
+    sc = None if dtype == BF else torch.full((2, nkv), 0.02, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    qn, kn = ((1 + .2 * torch.randn(hd, generator=g)).to(BF).cuda() for _ in "qk")
+    inv = (1e6 ** (-torch.arange(hd // 2, dtype=torch.float64) / (hd // 2))
+           ).float().cuda()
+    for n_new in ([20, 0, 3, 0], [1, 33, 1, 0], [-1, 1, 1, 5], [16, 1, 1, 1],
+                  [1, 1, -1, 60], [1, 1, 1, 1]):
+        code, p = d.step(n_new, 80)
+        assert code == 0
+        qkv = (torch.randn(80, (nq + 2 * nkv) * hd, generator=g) * 2).to(BF)
+        q = ops.paged_append(qkv.cuda(), pages, p.slot, p.pos, nq, qn, kn, EPS,
+                             inv, kv_scale=sc)
+        out = ops.paged_attention(q, pages, d.d_table, p.pos, req=p.req,
+                                  kv_scale=sc).cpu()
+        want, bound = P.attention(
+            q.cpu(), pages.cpu(), None if sc is None else sc.cpu(),
+            d.d_table.cpu(), p.req.tolist(), p.pos.tolist(), page, hd ** -0.5)
+        assert torch.isfinite(out).all()
+        assert ((out.double() - want).abs() <= bound).all()
+        n = sum(max(k, 0) for k in n_new)
+        # the keys that were appended are the ones the slots name
+        k = P.rope(qkv.reshape(80, -1, hd)[:n, nq:nq + nkv], kn.cpu(),
+                   p.pos.cpu()[:n], inv.cpu(), EPS)
+        s = p.slot.cpu()[:n].long()
+        got = pages.float().cpu()[s // page, 0, :, s % page].double()
+        if sc is not None:
+            got = got * 0.02
+        assert ((got - k).abs() <= 2.0 ** (-8 if dtype == BF else -4)
+                * k.abs() + 1e-3).all()
+    ops.check_status(torch.device("cuda", torch.cuda.current_device()))
