@@ -516,9 +516,9 @@ int slx_paged_append(const void* qkv, int64_t qkv_stride, int T, int n_q,
                      const int32_t* slot, const slx_kv_pages* pages,
                      void* q_out, int32_t* status, void* stream);
 
-/* Bytes of workspace slx_paged_attn_decode needs for T rows on the current
- * device.  Zero before the first call; every call leaves it reusable.  Calls
- * that may overlap (two streams, two graphs) need workspaces of their own. */
+/* Bytes of workspace slx_paged_attn_decode needs for T rows (the parts of
+ * rows that several CTAs share; 16-byte aligned, any content).  Calls that
+ * may overlap (two streams, two graphs) need workspaces of their own. */
 size_t slx_paged_attn_workspace_bytes(int T, int n_q, int n_kv, int head_dim);
 
 /* Attention of T rows over the pages (GQA, n_q / n_kv <= 16): row t attends

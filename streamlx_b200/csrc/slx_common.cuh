@@ -176,10 +176,10 @@ struct PerDevice {
   }
 };
 
-// <<<>>> replacement that adds the PDL attribute when pdl_enabled().
 template <typename... KArgs, typename... Args>
-cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block,
-                     size_t smem, cudaStream_t stream, Args... args) {
+cudaError_t launch_attr(bool pdl, void (*kernel)(KArgs...), dim3 grid,
+                        dim3 block, size_t smem, cudaStream_t stream,
+                        Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -189,8 +189,23 @@ cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block,
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// <<<>>> replacement that adds the PDL attribute when pdl_enabled().
+template <typename... KArgs, typename... Args>
+cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block,
+                     size_t smem, cudaStream_t stream, Args... args) {
+  return launch_attr(pdl_enabled(), kernel, grid, block, smem, stream, args...);
+}
+
+// The second launch of one call, as a PDL secondary of the first whatever
+// the caller's setting.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block,
+                           size_t smem, cudaStream_t stream, Args... args) {
+  return launch_attr(true, kernel, grid, block, smem, stream, args...);
 }
 
 // ------------------------------------------------------------------ MMA ---

@@ -369,21 +369,11 @@ def paged_append(qkv: torch.Tensor, pages: torch.Tensor, slot: torch.Tensor,
 
 def paged_workspace(rows: int, n_q: int, n_kv: int, head_dim: int,
                     device) -> torch.Tensor:
-    """Zeroed workspace of paged_attention for up to ``rows`` rows: calls
-    that may overlap (streams, graphs) need one each."""
-    with torch.cuda.device(device):
-        n = L.paged_attn_workspace_bytes(rows, n_q, n_kv, head_dim)
-        return torch.zeros(max(n, 16), dtype=torch.uint8, device=device)
-
-
-def _attn_workspace(need: int, device) -> torch.Tensor | None:
-    """Workspace of a call that was given none: one per stream (calls on a
-    stream do not overlap), or the graph's own inside a capture."""
-    if need == 0:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    return scratch(need, device, tag=("paged_attn", _raw_stream(device)))
+    """Workspace of paged_attention for up to ``rows`` rows, for callers
+    that must not allocate per call.  Its content does not matter; calls that
+    may overlap (streams, graphs) need one each."""
+    n = L.paged_attn_workspace_bytes(rows, n_q, n_kv, head_dim)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
 def paged_attention(q: torch.Tensor, pages: torch.Tensor,
@@ -428,8 +418,8 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor,
               "paged_attention: out must be contiguous bfloat16 [T, n_q, "
               "head_dim]")
     if workspace is None:
-        workspace = _attn_workspace(
-            L.paged_attn_workspace_bytes(T, n_q, pages.shape[2], hd), dev)
+        # the call's own: calls on other streams or in graphs share nothing
+        workspace = paged_workspace(T, n_q, pages.shape[2], hd, dev)
     else:
         _need(workspace.dtype == torch.uint8 and workspace.dim() == 1 and
               workspace.device == dev and workspace.is_contiguous(),

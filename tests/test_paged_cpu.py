@@ -42,6 +42,12 @@ def append(pages=None, **kw):
         None, None)
 
 
+@pytest.fixture(autouse=True)
+def no_error_left():
+    yield
+    assert attn(T=0) == 0       # a call that passes clears the message
+
+
 BAD_PAGES = [
     (dict(base=None), -1), (dict(base=PTR + 8), -1), (dict(dtype=2), -2),
     (dict(head_dim=96), -2), (dict(head_dim=256), -2), (dict(page_size=8), -2),
