@@ -525,8 +525,8 @@ size_t slx_paged_attn_workspace_bytes(int T, int n_q, int n_kv, int head_dim);
  * positions 0..pos[t] of request req[t] (req NULL: request t).
  * q [T][q_stride] bf16 (n_q heads of head_dim), out [T][n_q * head_dim]
  * bf16.  A row with pos < 0 gives zeros; a row with req or pos out of range
- * sets *status and gives zeros; keys on a page out of range set *status and
- * count as absent. */
+ * sets *status and gives zeros; keys and values on a page out of range set
+ * *status and read as zeros. */
 int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
                           const slx_kv_pages* pages, const int32_t* table,
                           int n_req, int max_pages, const int32_t* req,

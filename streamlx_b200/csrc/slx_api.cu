@@ -824,7 +824,7 @@ int pages_ok(const slx_kv_pages* p, const char* what, slx::KvPages* out) {
   if (p->dtype == SLX_KV_BF16 && (p->k_scale || p->v_scale))
     return fail(SLX_ERR_INVALID, "%s: bf16 pages take no scales", what);
   *out = {reinterpret_cast<uint8_t*>(p->base), p->k_scale, p->v_scale,
-          p->n_pages, ps, p->n_kv, p->head_dim};
+          p->n_pages, ps, p->n_kv, p->head_dim, __builtin_ctz(ps)};
   return SLX_OK;
 }
 

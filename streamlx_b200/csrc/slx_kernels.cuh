@@ -142,6 +142,7 @@ struct KvPages {
   const float* k_scale;
   const float* v_scale;
   int n_pages, page_size, n_kv, hd;
+  int page_shift;  // log2(page_size)
 };
 
 struct PlanArgs {

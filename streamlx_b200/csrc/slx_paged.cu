@@ -315,13 +315,18 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // of G q heads shares every key and value, so the bytes bound it: 2 G flops
 // per bf16 element.  The products still go to the tensor cores (G = 8 at HBM
 // speed would take most of the fp32 units' rate), as
-//   S^T [16 keys x 8 heads] = K [16 x hd] q^T,   O^T [hd x 8] += V^T P^T
+//   S^T [16 keys x 8 cols] = K [16 x hd] q^T,   O^T [hd x 8] += V^T P^T
 // with mma.m16n8k16: M is keys / dims, so no row is padding (tcgen05's
-// smallest M of 64 or 128 heads would be).  The contraction index of an MMA
-// may be permuted on both sides alike, and the fragments are chosen so that
-// each is 16 contiguous bytes of a key: keys and values go from global memory
-// to fragments without shared memory.  V pairs two keys per register (byte
-// permutes); S^T's accumulators become P^T's operand by movmatrix.
+// smallest M of 64 or 128 heads would be).  The columns are the q heads of
+// one row and, where they leave room, of the rows after it that belong to the
+// same request (a prompt's rows share their keys: see group_of).
+//
+// The contraction index of an MMA may be permuted on both sides alike; the
+// fragments are chosen so that each is 16 contiguous bytes of a key: keys and
+// values go from global memory to fragments without shared memory, the next
+// unit's into the registers that this one's have just left.  V pairs two keys
+// per register (byte permutes); S^T's accumulators become P^T's operand by
+// movmatrix.
 //
 // P is rounded to two 16-bit parts (hi + lo: 16 bits or more in all), so the
 // only rounding of note is the output's.  E4m3 keys and values become fp16
@@ -329,18 +334,19 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // element at 2^12 .. 2^13 (exact down to 2^-26 of it).
 //
 // Work is cut into units of 16 keys of one kv head; every CTA gets the same
-// number of consecutive units of the list (row, kv head, unit), whatever the
-// rows' lengths.  A (row, kv head) that one CTA covers is written directly,
-// the others leave (max, sum, O) parts that k_paged_join adds in order.
+// number of consecutive units of the list (row group, kv head, unit), whatever
+// the rows' lengths.  A (group, kv head) that one CTA covers
+// is written directly, the others leave (max, sum, O) parts that
+// k_paged_join adds in order.
 
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = 32 * kPaWarps;
-constexpr int kPaUnit = 16;
+constexpr int kPaUnit = 16;   // keys: what one MMA takes
 
 struct PaWork {       // workspace of one call
-  int4* desc;         // [n] split (row, kv head): first, last CTA, row, head
-  float* o;           // [2 CTAs][G][hd] parts: 2 w + 1 a segment's first
-  float2* ml;         // [2 CTAs][G] max (log2), sum
+  int4* desc;         // [n] split (group, kv head): first, last CTA, row, head
+  float* o;           // [2 CTAs][cols][hd] parts: 2 w + 1 a segment's first
+  float2* ml;         // [2 CTAs][cols] max (log2), sum; sum -1: no such row
 };
 
 SLX_DEV float exp2_fast(float x) {
@@ -349,17 +355,14 @@ SLX_DEV float exp2_fast(float x) {
   return y;
 }
 
-SLX_DEV uint4 ld_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-SLX_DEV uint2 ld_stream8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v2.u32 {%0,%1}, [%2];"
-               : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+template <int B>
+SLX_DEV void ld_stream(const uint8_t* p, uint32_t* v) {
+  if constexpr (B == 16)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
+  else
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+                 : "=r"(v[0]), "=r"(v[1]) : "l"(p));
 }
 
 template <bool BF16>
@@ -383,52 +386,121 @@ SLX_DEV uint32_t transpose8x8(uint32_t a) {
   return d;
 }
 
-// two e4m3 bytes -> fp16 pair (exact; NaN stays NaN)
-SLX_DEV uint32_t e4m3x2(uint32_t w) {
-  uint32_t d;
-  asm("{.reg .b16 t, u; mov.b32 {t, u}, %1; cvt.rn.f16x2.e4m3x2 %0, t;}"
-      : "=r"(d) : "r"(w));
-  return d;
+// four e4m3 bytes -> two fp16 pairs (exact; NaN stays NaN)
+SLX_DEV void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 t, u; mov.b32 {t, u}, %2; cvt.rn.f16x2.e4m3x2 %0, t; "
+      "cvt.rn.f16x2.e4m3x2 %1, u;}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
-// Keys row t attends: pos + 1, 0 for an idle row or one out of range.
-SLX_DEV int row_keys(const PagedAttnArgs& a, int t) {
-  const int p = a.pos[t];
-  if (p < 0) return 0;
-  const int r = a.req ? a.req[t] : t;
-  if (r < 0 || r >= a.n_req || p / a.kv.page_size >= a.max_pages) return 0;
-  return p + 1;
+SLX_DEV uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+// Row t's request and the keys it attends: pos + 1, 0 for an idle row or one
+// out of range.  (Both are read at once: rows are read in batches.)
+struct RowKeys {
+  int req, pos, keys;
+};
+SLX_DEV RowKeys row_keys(const PagedAttnArgs& a, int t) {
+  RowKeys r = {0, -1, 0};
+  if (t < a.T) {
+    r.pos = a.pos[t];
+    r.req = a.req ? a.req[t] : t;
+  }
+  const bool ok = (unsigned)r.req < (unsigned)a.n_req &&
+                  (unsigned)r.pos >> a.kv.page_shift < (unsigned)a.max_pages && r.pos >= 0;
+  r.keys = ok ? r.pos + 1 : 0;
+  return r;
+}
+
+// Rows are taken in aligned blocks of `rpb` (1, 2, 4 or 8: what fits the MMA's
+// columns); within one, consecutive rows of the same request form a group.
+// For a warp over rows t0 .. t0 + 31 (t0 a multiple of 32; n and r its rows'
+// keys and requests): the keys of the group that row t0 + lane leads, 0 if it
+// leads none.
+SLX_DEV int lead_keys(int n, int r, int rpb) {
+  if (rpb == 1) return n;
+  const int lane = threadIdx.x & 31;
+  const int before = __shfl_up_sync(0xffffffffu, r, 1);
+  const bool first = lane % rpb == 0 || before != r;
+  bool same = true;
+  int most = n;
+  for (int d = 1; d < rpb; ++d) {
+    const int rd = __shfl_down_sync(0xffffffffu, r, d);
+    const int nd = __shfl_down_sync(0xffffffffu, n, d);
+    same = same && lane % rpb + d < rpb && rd == r;
+    if (same) most = max(most, nd);
+  }
+  return first ? most : 0;
+}
+
+// Sum of 0 <= n <= 2^27 over a warp.
+SLX_DEV long long warp_sum(int n) {
+  return (long long)__reduce_add_sync(0xffffffffu, (unsigned)n & 0xffffu) +
+         ((long long)__reduce_add_sync(0xffffffffu, (unsigned)n >> 16) << 16);
+}
+
+// A run of units of one (row group, kv head) that falls to this CTA.
+struct PaSeg {
+  int row, kh, u0, u1, units, keys;
+};
 
 template <int HD, bool E4M3, int NT>
-__global__ void __launch_bounds__(kPaThreads) k_paged_attn(const PagedAttnArgs a,
-                                                           const PaWork ws) {
+__global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
+    k_paged_attn(const PagedAttnArgs a, const PaWork ws, int rpb) {
   constexpr int ES = E4M3 ? 1 : 2;       // bytes per element
-  constexpr int KQ = HD * ES / 64;       // 16-byte pieces of a key per lane
+  constexpr int RB = HD * ES;            // a key's row
+  constexpr int KQ = RB / 64;            // 16-byte pieces of a key per lane
   constexpr int KS = HD / 16;            // MMA steps of q . k
   constexpr int MT = HD / 16;            // 16-dim tiles of O^T
-  constexpr int PAD = HD + 4;
+  constexpr int VB = RB >= 128 ? 16 : 8; // bytes of a piece of V
+  constexpr int VP = RB / (8 * VB);      // its pieces per key
+  constexpr int VW = RB / 32;            // words per lane and key
+  // merging the warps' states: two of them at a time, as they lie in registers
+  __shared__ float4 s_acc[kPaWarps / 2][NT * MT * 32];
+  __shared__ float s_ml[2][2][8 * NT];
   __shared__ long long s_pre[kPaThreads + 1];
   __shared__ long long w_sum[kPaWarps];
-  __shared__ int s_chunk;
-  __shared__ float s_m[kPaWarps][8 * NT], s_l[kPaWarps][8 * NT];
-  __shared__ __align__(16) float s_o[kPaWarps][8 * NT][PAD];
+  __shared__ int s_run;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int w = blockIdx.x, nw = gridDim.x;
   const int nkv = a.kv.n_kv, G = a.nq / nkv, ps = a.kv.page_size;
-  const int sh = 31 - __clz(ps);
+  const int cols = rpb * G;
+  const int sh = a.kv.page_shift;
   const bool by_row = (long long)a.T * nkv <= nw;  // how desc is indexed
   pdl_launch_dependents();
   pdl_wait_primary();
-  // units before each thread's block of rows
-  const int chunk = (a.T + kPaThreads - 1) / kPaThreads;
-  {
-    long long n = 0;
-    const int t1 = min((tid + 1) * chunk, a.T);
-    for (int t = tid * chunk; t < t1; ++t)
-      n += (row_keys(a, t) + kPaUnit - 1) / kPaUnit;
-    long long v = n;
+  auto units_of = [](int keys) { return (int)(((unsigned)keys + kPaUnit - 1) / kPaUnit); };
+  // units before each of 128 runs of `run` tiles of 32 rows
+  const int tiles = (a.T + 31) / 32, run = (tiles + kPaThreads - 1) / kPaThreads;
+  RowKeys rk;                             // of row rb + lane
+  int len_l = 0;                          // keys of the group it leads
+  long long total;
+  if (tiles == 1) {
+    rk = row_keys(a, lane);
+    len_l = lead_keys(rk.keys, rk.req, rpb);
+    total = warp_sum(units_of(len_l)) * nkv;
+  } else {
+    s_pre[tid + 1] = 0;
+    __syncthreads();
+    constexpr int B = 4;  // tiles whose rows are read together
+    for (int i0 = warp * B; i0 < tiles; i0 += B * kPaWarps) {
+      RowKeys r[B];
+#pragma unroll
+      for (int j = 0; j < B; ++j) r[j] = row_keys(a, (i0 + j) * 32 + lane);
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const long long v = warp_sum(units_of(lead_keys(r[j].keys, r[j].req, rpb)));
+        if (lane == 0 && i0 + j < tiles)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s_pre[(i0 + j) / run + 1]),
+                    (unsigned long long)v);
+      }
+    }
+    __syncthreads();
+    long long v = s_pre[tid + 1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long u = __shfl_up_sync(0xffffffffu, v, o);
@@ -439,90 +511,180 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attn(const PagedAttnArgs a
     for (int i = 0; i < warp; ++i) v += w_sum[i];
     s_pre[tid + 1] = v;
     if (tid == 0) s_pre[0] = 0;
+    __syncthreads();
+    total = s_pre[kPaThreads] * nkv;
   }
-  // idle rows: zeros (and the status of those out of range)
-  for (int t = w; t < a.T; t += nw) {
-    if (row_keys(a, t) > 0) continue;
-    if (a.pos[t] >= 0 && tid == 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
-    uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)t * a.nq * HD);
-    for (int i = tid; i < a.nq * HD / 8; i += kPaThreads) o[i] = make_uint4(0, 0, 0, 0);
-    if (by_row)
-      for (int i = tid; i < nkv; i += kPaThreads) ws.desc[t * nkv + i] = make_int4(-1, 0, 0, 0);
-  }
-  __syncthreads();
-  const long long total = s_pre[kPaThreads] * nkv;
   // units per CTA: a multiple of the warps (a step is one unit per warp)
-  long long per = (total + nw - 1) / nw;
+  long long per = total < 0x7fffffff - nw ? ((unsigned)total + nw - 1) / (unsigned)nw
+                                          : (total + nw - 1) / nw;
   per = (per + kPaWarps - 1) / kPaWarps * kPaWarps;
   if (per < kPaWarps) per = kPaWarps;
   long long x = w * per;
   const long long x_end = min(x + per, total);
   int4 my_desc = make_int4(-1, 0, 0, 0);
   if (x < x_end) {
-    // the row unit x is in: its block of rows, then 32 rows at a time
-    if (s_pre[tid] * nkv <= x && x < s_pre[tid + 1] * nkv) s_chunk = tid;
-    __syncthreads();
-    int rb = s_chunk * chunk;             // first row of the warp's 32
-    long long before = s_pre[s_chunk] * nkv;
-    int row = -1, keys, units, len_l;     // len_l: keys of row rb + lane
-    for (;; rb += 32) {
-      len_l = rb + lane < a.T ? row_keys(a, rb + lane) : 0;
-      const int n = (len_l + kPaUnit - 1) / kPaUnit;
-      long long v = n;
+    PaSeg sg;
+    int rb = 0, req;
+    {
+      // the group unit x is in: its run of tiles, then tile by tile
+      long long before = 0;
+      if (tiles > 1) {
+        if (s_pre[tid] * nkv <= x && x < s_pre[tid + 1] * nkv) s_run = tid;
+        __syncthreads();
+        rb = s_run * run * 32;
+        before = s_pre[s_run] * nkv;
+      }
+      for (;; rb += 32) {
+        if (tiles > 1) {
+          rk = row_keys(a, rb + lane);
+          len_l = lead_keys(rk.keys, rk.req, rpb);
+        }
+        const int n = units_of(len_l);
+        long long v = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long u = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += u;
+        }
+        const bool here = before + (v - n) * nkv <= x && x < before + v * nkv;
+        const unsigned hit = __ballot_sync(0xffffffffu, here);
+        if (hit) {
+          const int i = __ffs(hit) - 1;
+          sg.row = rb + i;
+          before += (__shfl_sync(0xffffffffu, v, i) - __shfl_sync(0xffffffffu, n, i)) * nkv;
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, v, 31) * nkv;
       }
-      const bool here = before + (v - n) * nkv <= x && x < before + v * nkv;
-      const unsigned hit = __ballot_sync(0xffffffffu, here);
-      if (hit) {
-        const int i = __ffs(hit) - 1;
-        row = rb + i;
-        before += (__shfl_sync(0xffffffffu, v, i) - __shfl_sync(0xffffffffu, n, i)) * nkv;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, v, 31) * nkv;
+      sg.keys = __shfl_sync(0xffffffffu, len_l, sg.row - rb);
+      req = __shfl_sync(0xffffffffu, rk.req, sg.row - rb);
+      sg.units = units_of(sg.keys);
+      const long long in = x - before;
+      sg.kh = in < 0x7fffffff ? (int)((unsigned)in / (unsigned)sg.units)
+                              : (int)(in / sg.units);
+      sg.u0 = (int)(in - (long long)sg.kh * sg.units);
+      sg.u1 = (int)min((long long)sg.units, sg.u0 + (x_end - x));
     }
-    keys = __shfl_sync(0xffffffffu, len_l, row - rb);
-    units = (keys + kPaUnit - 1) / kPaUnit;
-    int kh = (int)((x - before) / units);
-    int u0 = (int)((x - before) % units);
-    while (true) {
-      const int u1 = (int)min((long long)units, u0 + (x_end - x));
-      const int req = a.req ? a.req[row] : row;
-      const int32_t* tab = a.table + (size_t)req * a.max_pages;
-      // q^T fragments of the group's heads
-      uint32_t qf[NT][KS][2];
-      float fac[NT][2];  // of heads 2c, 2c + 1: scores in log2 units
-      const float fs = a.scale * 1.4426950408889634f * (E4M3 ? a.kv.k_scale[kh] : 1.f);
+    const size_t page_bytes = (size_t)2 * nkv * ps * RB, v_off = (size_t)nkv * ps * RB;
+    // this lane's pieces of keys g, g + 8 and of values 2c, 2c + 1, 2c + 8, 2c + 9
+    uint32_t kr[2][KQ][4], vr[4][VW];
+    const int k_at = g * RB + c * 16, v_at = 2 * c * RB + g * VB;
+    const int32_t* tab = nullptr;
+    const uint8_t* head = nullptr;        // the kv head's keys in page 0
+    auto segment = [&] {
+      tab = a.table + (size_t)req * a.max_pages;
+      head = a.kv.base + (size_t)sg.kh * ps * RB;
+    };
+    // page of unit u of the segment (-1 behind its end)
+    auto page_of = [&](int u) { return u < sg.u1 ? tab[(u * kPaUnit) >> sh] : -1; };
+    auto keys_at = [&](int u, int page) {
+      return head + (size_t)(unsigned)page * page_bytes + ((u * kPaUnit) & (ps - 1)) * RB;
+    };
+    // A unit's last key held by the group, -1 for a page out of range (zeros).
+    auto last_of = [&](int u, int page) {
+      if ((unsigned)page < (unsigned)a.kv.n_pages) return min(kPaUnit, sg.keys - u * kPaUnit) - 1;
+      if (lane == 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+      return -1;
+    };
+    auto load_k = [&](int u, int page) {
+      const int last = last_of(u, page);
+      if (last == kPaUnit - 1) {
+        const uint8_t* p = keys_at(u, page) + k_at;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int h = nt * 8 + g;
-        const uint8_t* qp = reinterpret_cast<const uint8_t*>(
-            a.q + (size_t)row * a.q_stride + (size_t)(kh * G + h) * HD);
-        if constexpr (!E4M3) {
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int q = 0; q < KQ; ++q) ld_stream<16>(p + r * 8 * RB + q * 64, kr[r][q]);
+      } else {
+        const uint8_t* p = keys_at(u, last < 0 ? 0 : page) + c * 16;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int q = 0; q < KQ; ++q) {
-            const uint4 v = h < G ? *reinterpret_cast<const uint4*>(qp + q * 64 + c * 16)
-                                  : make_uint4(0, 0, 0, 0);
-            qf[nt][2 * q][0] = v.x;
-            qf[nt][2 * q][1] = v.y;
-            qf[nt][2 * q + 1][0] = v.z;
-            qf[nt][2 * q + 1][1] = v.w;
+            kr[r][q][0] = kr[r][q][1] = kr[r][q][2] = kr[r][q][3] = 0;
+            if (g + 8 * r <= last) ld_stream<16>(p + (g + 8 * r) * RB + q * 64, kr[r][q]);
+          }
+      }
+    };
+    auto load_v = [&](int u, int page) {
+      const int last = last_of(u, page);
+      if (last == kPaUnit - 1) {
+        const uint8_t* p = keys_at(u, page) + v_off + v_at;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int q = 0; q < VP; ++q)
+            ld_stream<VB>(p + ((r & 1) + 8 * (r >> 1)) * RB + q * 128, vr[r] + q * (VB / 4));
+      } else {
+        const uint8_t* p = keys_at(u, last < 0 ? 0 : page) + v_off + g * VB;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = 2 * c + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+          for (int q = 0; q < VW; ++q) vr[r][q] = 0;
+          if (key <= last) {
+#pragma unroll
+            for (int q = 0; q < VP; ++q) ld_stream<VB>(p + key * RB + q * 128, vr[r] + q * (VB / 4));
+          }
+        }
+      }
+    };
+    segment();
+    int page = page_of(sg.u0 + warp);
+    bool loaded = false;                  // the first unit is on its way
+    while (true) {
+      int u = sg.u0 + warp;
+      // columns n of the MMAs: row n / G of the group, q head n % G
+      uint32_t qf[NT][KS][2];
+      float fac[NT][2];  // of columns 2c, 2c + 1: scores in log2 units
+      int lim[NT][2];    // their keys (0: no such row)
+      const float fs = a.scale * 1.4426950408889634f * (E4M3 ? a.kv.k_scale[sg.kh] : 1.f);
+      uint4 qv[NT][HD / 32];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int n = nt * 8 + g;
+        int row = sg.row, keys = n < cols ? sg.keys : 0;
+        if (rpb > 1) {
+          row += n / G;
+          const RowKeys r = row_keys(a, row);
+          keys = n < cols && row / rpb == sg.row / rpb && r.req == req ? r.keys : 0;
+        }
+        lim[nt][0] = __shfl_sync(0xffffffffu, keys, 8 * c);
+        lim[nt][1] = __shfl_sync(0xffffffffu, keys, 8 * c + 4);
+        const uint8_t* qp = reinterpret_cast<const uint8_t*>(
+            a.q + (size_t)(keys ? row : sg.row) * a.q_stride +
+            (size_t)(sg.kh * G + n % G) * HD);
+        // bf16 pages: 8 dims of each 32; e4m3: 16 of each 64 (as the keys')
+#pragma unroll
+        for (int q = 0; q < HD / 32; ++q)
+          qv[nt][q] = keys > 0 ? *reinterpret_cast<const uint4*>(
+                                     qp + (E4M3 ? (q >> 1) * 128 + c * 32 + (q & 1) * 16
+                                                : q * 64 + c * 16))
+                               : make_uint4(0, 0, 0, 0);
+      }
+      if (u < sg.u1 && !loaded) {
+        load_k(u, page);
+        load_v(u, page);
+      }
+      page = page_of(u + kPaWarps);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (!E4M3) {
+#pragma unroll
+          for (int q = 0; q < HD / 32; ++q) {
+            qf[nt][2 * q][0] = qv[nt][q].x;
+            qf[nt][2 * q][1] = qv[nt][q].y;
+            qf[nt][2 * q + 1][0] = qv[nt][q].z;
+            qf[nt][2 * q + 1][1] = qv[nt][q].w;
           }
           fac[nt][0] = fac[nt][1] = fs;
         } else {
-          uint4 v[2 * KQ];
           float mx = 0.f;
 #pragma unroll
-          for (int q = 0; q < 2 * KQ; ++q) {
-            v[q] = h < G ? *reinterpret_cast<const uint4*>(qp + (q >> 1) * 128 + c * 32 + (q & 1) * 16)
-                         : make_uint4(0, 0, 0, 0);
-            const uint32_t u[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+          for (int q = 0; q < HD / 32; ++q) {
+            const uint32_t v[4] = {qv[nt][q].x, qv[nt][q].y, qv[nt][q].z, qv[nt][q].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(u[i])), fabsf(bf16_hi(u[i]))));
+              mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(v[i])), fabsf(bf16_hi(v[i]))));
           }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -532,16 +694,26 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attn(const PagedAttnArgs a
           const float up = __uint_as_float((uint32_t)(127 + k) << 23);
           const float down = __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
-          for (int q = 0; q < 2 * KQ; ++q) {
-            const uint32_t u[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+          for (int q = 0; q < HD / 32; ++q) {
+            const uint32_t v[4] = {qv[nt][q].x, qv[nt][q].y, qv[nt][q].z, qv[nt][q].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              qf[nt][2 * q + (i >> 1)][i & 1] = pack_f16x2(bf16_lo(u[i]) * up, bf16_hi(u[i]) * up);
+              qf[nt][2 * q + (i >> 1)][i & 1] = pack_f16x2(bf16_lo(v[i]) * up, bf16_hi(v[i]) * up);
           }
-          // lane 8c holds head 2c's factor, lane 8c + 4 head 2c + 1's
+          // lane 8c holds column 2c's factor, lane 8c + 4 column 2c + 1's
           fac[nt][0] = fs * __shfl_sync(0xffffffffu, down, 8 * c);
           fac[nt][1] = fs * __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }
+      }
+      // keys that every row of the group attends
+      int common = sg.keys;
+      if (rpb > 1) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (lim[nt][i]) common = min(common, lim[nt][i]);
+        common = __reduce_min_sync(0xffffffffu, common);
       }
       float acc[NT][MT][4];
       float m[NT][2], l[NT][2];
@@ -553,92 +725,57 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attn(const PagedAttnArgs a
         for (int i = 0; i < MT; ++i)
           acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
       }
-      const size_t v_off = (size_t)nkv * ps * HD * ES;
-      int u = u0 + warp;
-      int page = u < u1 ? tab[(u * kPaUnit) >> sh] : 0;
-      for (; u < u1; u += kPaWarps) {
+      for (; u < sg.u1; u += kPaWarps) {
         const int k0 = u * kPaUnit;
-        const int next = u + kPaWarps < u1 ? tab[((u + kPaWarps) * kPaUnit) >> sh] : 0;
-        if (page < 0 || page >= a.kv.n_pages) {
-          if (lane == 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
-          page = next;
-          continue;
-        }
-        const int last = min(kPaUnit, keys - k0) - 1;  // last key held
-        const uint8_t* kp = a.kv.base +
-            (((size_t)page * 2 * nkv + kh) * ps + (k0 & (ps - 1))) * (HD * ES);
-        const uint8_t* vp = kp + v_off;
-        page = next;
-        uint4 kr[2][KQ];
+        float s[NT][4], s2[NT][4];  // even and odd steps: two shorter chains
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint8_t* p = kp + min(g + 8 * r, last) * (HD * ES) + c * 16;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int q = 0; q < KQ; ++q) kr[r][q] = ld_stream(p + q * 64);
-        }
-        // value words of keys 2c, 2c + 1, 2c + 8, 2c + 9
-        constexpr int VW = HD * ES / 32;  // words per lane and key
-        uint32_t vr[4][VW];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = 2 * c + (r & 1) + 8 * (r >> 1);
-          const uint8_t* p = vp + min(key, last) * (HD * ES) + g * (VW >= 4 ? 16 : 8);
-          if constexpr (VW >= 4) {
-#pragma unroll
-            for (int q = 0; q < VW / 4; ++q) {
-              const uint4 v = ld_stream(p + q * 128);
-              vr[r][4 * q] = v.x;
-              vr[r][4 * q + 1] = v.y;
-              vr[r][4 * q + 2] = v.z;
-              vr[r][4 * q + 3] = v.w;
-            }
-          } else {
-            const uint2 v = ld_stream8(p);
-            vr[r][0] = v.x;
-            vr[r][1] = v.y;
-          }
-          if (last < kPaUnit - 1 && key > last) {
-#pragma unroll
-            for (int q = 0; q < VW; ++q) vr[r][q] = 0;
-          }
-        }
-        float s[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+          for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
 #pragma unroll
         for (int q = 0; q < KQ; ++q) {
-          const uint32_t lo[4] = {kr[0][q].x, kr[0][q].y, kr[0][q].z, kr[0][q].w};
-          const uint32_t hi[4] = {kr[1][q].x, kr[1][q].y, kr[1][q].z, kr[1][q].w};
+          const uint32_t(&lo)[4] = kr[0][q];
+          const uint32_t(&hi)[4] = kr[1][q];
           if constexpr (!E4M3) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816<true>(s[nt], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1],
-                               qf[nt][2 * q + i][0], qf[nt][2 * q + i][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<true>(s[nt], lo[0], hi[0], lo[1], hi[1], qf[nt][2 * q][0], qf[nt][2 * q][1]);
+              mma16816<true>(s2[nt], lo[2], hi[2], lo[3], hi[3], qf[nt][2 * q + 1][0],
+                             qf[nt][2 * q + 1][1]);
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t a0 = e4m3x2(lo[i]), a2 = e4m3x2(lo[i] >> 16);
-              const uint32_t a1 = e4m3x2(hi[i]), a3 = e4m3x2(hi[i] >> 16);
+              uint32_t a0, a1, a2, a3;
+              e4m3x4(lo[i], a0, a2);
+              e4m3x4(hi[i], a1, a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma16816<false>(s[nt], a0, a1, a2, a3, qf[nt][4 * q + i][0],
+                mma16816<false>(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][4 * q + i][0],
                                 qf[nt][4 * q + i][1]);
             }
           }
         }
+        const int pg = page;
+        const bool more_u = u + kPaWarps < sg.u1;
+        if (more_u) {
+          load_k(u + kPaWarps, pg);
+          page = page_of(u + 2 * kPaWarps);
+        }
         uint32_t ph[NT][2], pl[NT][2];  // P^T operands: hi and lo parts
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float p[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            p[i] = g + 8 * (i >> 1) <= last ? s[nt][i] * fac[nt][i & 1] : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * fac[nt][i & 1];
+          if (k0 + kPaUnit > common) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (k0 + 8 * (i >> 1) + g >= lim[nt][i & 1]) s[nt][i] = -INFINITY;
+          }
           float f[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float mx = fmaxf(p[i], p[i + 2]);
+            float mx = fmaxf(s[nt][i], s[nt][i + 2]);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -646,9 +783,9 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attn(const PagedAttnArgs a
             const float ms = mx == -INFINITY ? 0.f : mx;
             f[i] = exp2_fast(m[nt][i] - ms);
             m[nt][i] = mx;
-            p[i] = exp2_fast(p[i] - ms);
-            p[i + 2] = exp2_fast(p[i + 2] - ms);
-            l[nt][i] = l[nt][i] * f[i] + (p[i] + p[i + 2]);
+            s[nt][i] = exp2_fast(s[nt][i] - ms);
+            s[nt][i + 2] = exp2_fast(s[nt][i + 2] - ms);
+            l[nt][i] = l[nt][i] * f[i] + (s[nt][i] + s[nt][i + 2]);
           }
           if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
@@ -660,197 +797,347 @@ __global__ void __launch_bounds__(kPaThreads) k_paged_attn(const PagedAttnArgs a
             }
           }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int r = 0; r < 2; ++r) {
+            const float p0 = s[nt][2 * r], p1 = s[nt][2 * r + 1];
             uint32_t hi, lo;
             if constexpr (!E4M3) {
-              hi = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-              lo = pack_bf16x2(p[2 * i] - bf16_lo(hi), p[2 * i + 1] - bf16_hi(hi));
+              hi = pack_bf16(p0, p1);
+              lo = pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
             } else {
-              hi = pack_f16x2(p[2 * i], p[2 * i + 1]);
+              hi = pack_f16x2(p0, p1);
               const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              lo = pack_f16x2(p[2 * i] - b.x, p[2 * i + 1] - b.y);
+              lo = pack_f16x2(p0 - b.x, p1 - b.y);
             }
-            ph[nt][i] = transpose8x8(hi);
-            pl[nt][i] = transpose8x8(lo);
+            ph[nt][r] = transpose8x8(hi);
+            pl[nt][r] = transpose8x8(lo);
           }
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint32_t a0, a1, a2, a3;
+        // V^T fragments of tile i
+        auto frag = [&](int i, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3,
+                        uint32_t (&f)[4]) {
           if constexpr (!E4M3) {
             // word i of the lane's dims: dims 2i (low halves) and 2i + 1
-            a0 = __byte_perm(vr[0][i], vr[1][i], 0x5410);
-            a1 = __byte_perm(vr[0][i], vr[1][i], 0x7632);
-            a2 = __byte_perm(vr[2][i], vr[3][i], 0x5410);
-            a3 = __byte_perm(vr[2][i], vr[3][i], 0x7632);
+            f[0] = __byte_perm(v0, v1, 0x5410);
+            f[1] = __byte_perm(v0, v1, 0x7632);
+            f[2] = __byte_perm(v2, v3, 0x5410);
+            f[3] = __byte_perm(v2, v3, 0x7632);
           } else {
             // bytes 2 (i % 2), + 1 of word i / 2: dims 2i and 2i + 1
             const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
-            const uint32_t lo = __byte_perm(vr[0][i >> 1], vr[1][i >> 1], sel);
-            const uint32_t hi = __byte_perm(vr[2][i >> 1], vr[3][i >> 1], sel);
-            a0 = e4m3x2(lo);
-            a1 = e4m3x2(lo >> 16);
-            a2 = e4m3x2(hi);
-            a3 = e4m3x2(hi >> 16);
+            e4m3x4(__byte_perm(v0, v1, sel), f[0], f[1]);
+            e4m3x4(__byte_perm(v2, v3, sel), f[2], f[3]);
           }
+        };
+        constexpr int D = E4M3 ? 2 : 1;
+        // a weight of 0 does not hide an infinite or NaN value from a row
+        // that does not attend it: such keys go row by row
+        bool apart = false;
+        if (rpb > 1 && k0 + kPaUnit > common) {
+          bool odd = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<!E4M3>(acc[nt][i], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-            mma16816<!E4M3>(acc[nt][i], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int q = 0; q < VW; ++q) {
+              const uint32_t v = vr[r][q];
+              if constexpr (!E4M3)
+                odd |= (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
+              else
+                odd |= ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            }
+          apart = __any_sync(0xffffffffu, odd);
+        }
+        if (!apart) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            uint32_t f[4];
+            frag(i, vr[0][i / D], vr[1][i / D], vr[2][i / D], vr[3][i / D], f);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<!E4M3>(acc[nt][i], f[0], f[1], f[2], f[3], ph[nt][0], ph[nt][1]);
+              mma16816<!E4M3>(acc[nt][i], f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
+            }
+          }
+        } else {
+          for (int j = 0; j < rpb; ++j) {
+            const int row = sg.row + j;
+            const RowKeys rj = row_keys(a, row);
+            if (row >= a.T || row / rpb != sg.row / rpb || rj.req != req) break;
+            const int at = k0 + 2 * c, keys = rj.keys;
+            const bool on[4] = {at < keys, at + 1 < keys, at + 8 < keys, at + 9 < keys};
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              uint32_t f[4];
+              frag(i, on[0] ? vr[0][i / D] : 0, on[1] ? vr[1][i / D] : 0,
+                   on[2] ? vr[2][i / D] : 0, on[3] ? vr[3][i / D] : 0, f);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816<!E4M3>(t, f[0], f[1], f[2], f[3], ph[nt][0], ph[nt][1]);
+                mma16816<!E4M3>(t, f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if ((nt * 8 + 2 * c + (k & 1)) / G == j) acc[nt][i][k] += t[k];
+              }
+            }
           }
         }
+        if (more_u) load_v(u + kPaWarps, pg);
       }
-      // the warps' states into shared memory: O in dim order per head
+      // the next segment's first unit is on its way while this one's states
+      // are merged
+      const PaSeg done = sg;
+      const long long x0 = x;
+      x += sg.u1 - sg.u0;
+      const bool more = x < x_end;
+      if (more) {
+        sg.u0 = 0;
+        if (++sg.kh == nkv) {
+          sg.kh = 0;
+          unsigned hit = __ballot_sync(0xffffffffu, len_l > 0 && rb + lane > sg.row);
+          while (!hit) {  // there is one: x < total
+            rb += 32;
+            rk = row_keys(a, rb + lane);
+            len_l = lead_keys(rk.keys, rk.req, rpb);
+            hit = __ballot_sync(0xffffffffu, len_l > 0);
+          }
+          sg.row = rb + __ffs(hit) - 1;
+          sg.keys = __shfl_sync(0xffffffffu, len_l, sg.row - rb);
+          req = __shfl_sync(0xffffffffu, rk.req, sg.row - rb);
+          sg.units = units_of(sg.keys);
+        }
+        sg.u1 = (int)min((long long)sg.units, x_end - x);
+        segment();
+        page = page_of(warp);
+      }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float v = l[nt][i];
-          v += __shfl_xor_sync(0xffffffffu, v, 4);
-          v += __shfl_xor_sync(0xffffffffu, v, 8);
-          v += __shfl_xor_sync(0xffffffffu, v, 16);
-          const int h = nt * 8 + 2 * c + i;
-          if (g == 0) {
-            s_m[warp][h] = m[nt][i];
-            s_l[warp][h] = v;
-          }
+          l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 4);
+          l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 8);
+          l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], 16);
+        }
+      // warps 2, 3 into 0, 1, then 1 into 0
 #pragma unroll
-          for (int j = 0; j < MT; j += 2) {
-            // tiles j, j + 1: four consecutive dims
-            const int d = E4M3 ? g * (HD / 8) + 2 * j : (j / 4) * 64 + g * 8 + (j % 4) * 2;
-            *reinterpret_cast<float4*>(&s_o[warp][h][d]) = make_float4(
-                acc[nt][j][i], acc[nt][j][i + 2], acc[nt][j + 1][i], acc[nt][j + 1][i + 2]);
+      for (int half = kPaWarps / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp >= half && warp < 2 * half) {
+          float4* d = s_acc[warp - half] + lane;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+              d[(nt * MT + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1],
+                                                  acc[nt][i][2], acc[nt][i][3]);
+            if (g == 0) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                s_ml[warp - half][0][nt * 8 + 2 * c + i] = m[nt][i];
+                s_ml[warp - half][1][nt * 8 + 2 * c + i] = l[nt][i];
+              }
+            }
+          }
+        }
+        __syncthreads();
+        if (half == kPaWarps / 2) {
+          loaded = more && warp < sg.u1;
+          if (loaded) {
+            load_k(warp, page);
+            load_v(warp, page);
+          }
+        }
+        if (warp < half) {
+          const float4* d = s_acc[warp] + lane;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float f0[2], f1[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float om = s_ml[warp][0][nt * 8 + 2 * c + i];
+              const float mx = fmaxf(m[nt][i], om);
+              const float ms = mx == -INFINITY ? 0.f : mx;
+              f0[i] = exp2_fast(m[nt][i] - ms);
+              f1[i] = exp2_fast(om - ms);
+              l[nt][i] = l[nt][i] * f0[i] + s_ml[warp][1][nt * 8 + 2 * c + i] * f1[i];
+              m[nt][i] = mx;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const float4 v = d[(nt * MT + i) * 32];
+              acc[nt][i][0] = acc[nt][i][0] * f0[0] + v.x * f1[0];
+              acc[nt][i][1] = acc[nt][i][1] * f0[1] + v.y * f1[1];
+              acc[nt][i][2] = acc[nt][i][2] * f0[0] + v.z * f1[0];
+              acc[nt][i][3] = acc[nt][i][3] * f0[1] + v.w * f1[1];
+            }
           }
         }
       }
-      __syncthreads();
-      const bool whole = u0 == 0 && u1 == units;
-      const int part = 2 * w + (u0 == 0 ? 1 : 0);
-      const float sv = E4M3 ? a.kv.v_scale[kh] : 1.f;
-      for (int i = tid; i < G * (HD / 4); i += kPaThreads) {
-        const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        float M = -INFINITY;
+      const bool whole = done.u0 == 0 && done.u1 == done.units;
+      if (warp == 0) {
+        const float sv = E4M3 ? a.kv.v_scale[done.kh] : 1.f;
+        const size_t part = 2 * (size_t)w + (done.u0 == 0 ? 1 : 0);
 #pragma unroll
-        for (int k = 0; k < kPaWarps; ++k) M = fmaxf(M, s_m[k][h]);
-        const float Mf = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < kPaWarps; ++k) {
-          const float f = exp2_fast(s_m[k][h] - Mf);
-          const float4 v = *reinterpret_cast<const float4*>(&s_o[k][h][d]);
-          L += f * s_l[k][h];
-          o.x += f * v.x;
-          o.y += f * v.y;
-          o.z += f * v.z;
-          o.w += f * v.w;
-        }
-        o.x *= sv;
-        o.y *= sv;
-        o.z *= sv;
-        o.w *= sv;
-        if (whole) {
-          *reinterpret_cast<uint2*>(a.out + ((size_t)row * a.nq + kh * G + h) * HD + d) =
-              make_uint2(pack_bf16x2(o.x / L, o.y / L), pack_bf16x2(o.z / L, o.w / L));
-        } else {
-          *reinterpret_cast<float4*>(ws.o + ((size_t)part * G + h) * HD + d) = o;
-          if (d == 0) ws.ml[(size_t)part * G + h] = make_float2(M, L);
-        }
+          for (int i = 0; i < 2; ++i) {
+            const int n = nt * 8 + 2 * c + i;
+            if (n >= cols) continue;
+            const float scale = whole ? sv / l[nt][i] : sv;
+            float* po = ws.o + (part * cols + n) * HD;
+            uint16_t* out = a.out + ((size_t)(done.row + n / G) * a.nq + done.kh * G + n % G) * HD;
+            if (!whole && g == 0)
+              ws.ml[part * cols + n] = make_float2(m[nt][i], lim[nt][i] ? l[nt][i] : -1.f);
+            if (lim[nt][i] == 0) continue;  // no such row
+#pragma unroll
+            for (int j = 0; j < MT; j += 2) {
+              // tiles j, j + 1: four consecutive dims
+              const int d = E4M3 ? g * (HD / 8) + 2 * j : (j / 4) * 64 + g * 8 + (j % 4) * 2;
+              const float4 o = make_float4(acc[nt][j][i] * scale, acc[nt][j][i + 2] * scale,
+                                           acc[nt][j + 1][i] * scale,
+                                           acc[nt][j + 1][i + 2] * scale);
+              if (whole)
+                *reinterpret_cast<uint2*>(out + d) =
+                    make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+              else
+                *reinterpret_cast<float4*>(po + d) = o;
+            }
+          }
       }
-      if (u0 == 0) {
+      if (done.u0 == 0) {
         const int4 d = whole ? make_int4(-1, 0, 0, 0)
-                             : make_int4(w, (int)((x + units - 1) / per), row, kh);
+                             : make_int4(w, (int)((x0 + done.units - 1) / per), done.row, done.kh);
         if (by_row) {
-          if (tid == 0) ws.desc[row * nkv + kh] = d;
+          if (tid == 0) ws.desc[done.row * nkv + done.kh] = d;
         } else if (!whole) {
           my_desc = d;
         }
       }
-      x += u1 - u0;
-      if (x >= x_end) break;
-      __syncthreads();  // s_o is read before the next segment's is written
-      u0 = 0;
-      if (++kh == nkv) {
-        kh = 0;
-        // the next row with keys (there is one: x < total)
-        unsigned more = __ballot_sync(0xffffffffu, len_l > 0 && rb + lane > row);
-        while (!more) {
-          rb += 32;
-          len_l = rb + lane < a.T ? row_keys(a, rb + lane) : 0;
-          more = __ballot_sync(0xffffffffu, len_l > 0);
-        }
-        row = rb + __ffs(more) - 1;
-        keys = __shfl_sync(0xffffffffu, len_l, row - rb);
-        units = (keys + kPaUnit - 1) / kPaUnit;
-      }
+      if (!more) break;
     }
   }
   if (!by_row && tid == 0) ws.desc[w] = my_desc;
+  // idle rows: zeros (and the status of those out of range)
+  if (warp != 0) return;
+  for (int i = w; i < tiles; i += nw) {
+    const int t = i * 32 + lane;
+    const RowKeys r = row_keys(a, t);
+    const int n = lead_keys(r.keys, r.req, rpb);
+    if (by_row && t < a.T && n == 0)
+      for (int k = 0; k < nkv; ++k) ws.desc[t * nkv + k] = make_int4(-1, 0, 0, 0);
+    const bool idle = t < a.T && r.keys == 0;
+    if (idle && r.pos >= 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+    for (unsigned todo = __ballot_sync(0xffffffffu, idle); todo; todo &= todo - 1) {
+      uint4* o = reinterpret_cast<uint4*>(
+          a.out + (size_t)(i * 32 + __ffs(todo) - 1) * a.nq * HD);
+      for (int k = lane; k < a.nq * HD / 8; k += 32) o[k] = make_uint4(0, 0, 0, 0);
+    }
+  }
 }
 
-// Parts of one split (row, kv head), one q head per CTA: added in order of
-// the keys, eight parts at a time per warp group.
-constexpr int kJoinThreads = 256;
+// Parts of one split (group, kv head) added in the order of the keys, a thread
+// per four dims of a column and NG parts side by side; each thread requests
+// eight parts before it uses one.  COL: one column per CTA (few segments of
+// many parts), else all columns (many segments of a few parts, and most CTAs
+// find nothing to do).
+constexpr int kJoinThreads = 512;
+constexpr int kJoinBatch = 8;
 
-template <int HD>
+template <int HD, bool COL>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedAttnArgs a,
-                                                             const PaWork ws) {
-  constexpr int TP = HD / 4;                 // threads per part
-  constexpr int NG = kJoinThreads / TP;      // parts at a time
-  __shared__ float s_red[kJoinThreads / 32];
-  __shared__ float s_l[NG];
-  __shared__ __align__(16) float s_o[NG][HD];
+                                                             const PaWork ws, int rpb) {
+  __shared__ __align__(16) float4 s_o[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
   pdl_launch_dependents();
   pdl_wait_primary();
   const int4 d = ws.desc[blockIdx.x];
   if (d.x < 0) return;
-  const int G = a.nq / a.kv.n_kv, h = blockIdx.y;
-  const int n = d.y - d.x + 1;
-  const int tid = threadIdx.x;
+  constexpr int TP = HD / 4;                 // threads per column
+  const int G = a.nq / a.kv.n_kv, cols = rpb * G;
+  const int width = COL ? TP : cols * TP;    // threads per part
+  const int NG = kJoinThreads / width;       // parts side by side
+  const int tid = threadIdx.x, q = tid / width;
+  const int n = COL ? blockIdx.y : tid % width / TP, d4 = tid % TP * 4;
+  const int parts = d.y - d.x + 1;
   // part i of the segment: the first CTA's second slot, then first slots
-  auto part = [&](int i) { return (size_t)(2 * (d.x + i) + (i == 0 ? 1 : 0)) * G + h; };
-  float M = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads) M = fmaxf(M, ws.ml[part(i)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if ((tid & 31) == 0) s_red[tid >> 5] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) M = fmaxf(M, s_red[i]);
-  if (M == -INFINITY) M = 0.f;
-  const int q = tid / TP, d4 = (tid % TP) * 4;
-  float L = 0.f;
+  auto part = [&](int i) { return (size_t)(2 * (d.x + i) + (i == 0 ? 1 : 0)) * cols + n; };
+  float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = q; i < n; i += NG) {
-    const size_t p = part(i);
-    const float2 ml = ws.ml[p];
-    const float4 v = *reinterpret_cast<const float4*>(ws.o + p * HD + d4);
-    const float f = exp2_fast(ml.x - M);
-    L += f * ml.y;
-    o.x += f * v.x;
-    o.y += f * v.y;
-    o.z += f * v.z;
-    o.w += f * v.w;
-  }
-  *reinterpret_cast<float4*>(&s_o[q][d4]) = o;
-  if (d4 == 0) s_l[q] = L;
-  __syncthreads();
-  if (tid < HD) {
-    float O = 0.f;
-    L = 0.f;
+  bool none = false;
+  for (int i0 = 0; i0 < parts && q < NG; i0 += NG * kJoinBatch) {
+    float2 ml[kJoinBatch];
+    float4 v[kJoinBatch];
+    float mx = M;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      O += s_o[i][tid];
-      L += s_l[i];
+    for (int j = 0; j < kJoinBatch; ++j) {
+      const int i = i0 + j * NG + q;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < parts) {
+        ml[j] = ws.ml[part(i)];
+        v[j] = *reinterpret_cast<const float4*>(ws.o + part(i) * HD + d4);
+      }
     }
-    a.out[((size_t)d.z * a.nq + d.w * G + h) * HD + tid] = f32_to_bf16(O / L);
+#pragma unroll
+    for (int j = 0; j < kJoinBatch; ++j) {
+      none |= ml[j].y == -1.f;               // the group has no such row
+      mx = fmaxf(mx, ml[j].x);
+    }
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    const float f0 = exp2_fast(M - ms);
+    L *= f0;
+    o.x *= f0;
+    o.y *= f0;
+    o.z *= f0;
+    o.w *= f0;
+    M = mx;
+#pragma unroll
+    for (int j = 0; j < kJoinBatch; ++j) {
+      const float f = exp2_fast(ml[j].x - ms);
+      L += f * ml[j].y;
+      o.x += f * v[j].x;
+      o.y += f * v[j].y;
+      o.z += f * v[j].z;
+      o.w += f * v[j].w;
+    }
   }
+  if (NG > 1) {
+    s_ml[tid] = make_float2(M, none ? -1.f : L);
+    s_o[tid] = o;
+    __syncthreads();
+    if (q > 0) return;
+    const int ng = min(NG, parts);
+    float mx = M;
+    for (int i = 1; i < ng; ++i) {
+      const float2 ml = s_ml[i * width + tid];
+      none |= ml.y == -1.f;
+      mx = fmaxf(mx, ml.x);
+    }
+    const float ms = mx == -INFINITY ? 0.f : mx, f0 = exp2_fast(M - ms);
+    L *= f0;
+    o.x *= f0;
+    o.y *= f0;
+    o.z *= f0;
+    o.w *= f0;
+#pragma unroll 4
+    for (int i = 1; i < ng; ++i) {
+      const float2 ml = s_ml[i * width + tid];
+      const float4 v = s_o[i * width + tid];
+      const float f = exp2_fast(ml.x - ms);
+      L += ml.y * f;
+      o.x += v.x * f;
+      o.y += v.y * f;
+      o.z += v.z * f;
+      o.w += v.w * f;
+    }
+  }
+  if (q > 0 || none) return;
+  *reinterpret_cast<uint2*>(a.out + ((size_t)(d.z + n / G) * a.nq + d.w * G + n % G) * HD + d4) =
+      make_uint2(pack_bf16(o.x / L, o.y / L), pack_bf16(o.z / L, o.w / L));
 }
 
 namespace {
 
-using AttnKernel = void (*)(PagedAttnArgs, PaWork);
+using AttnKernel = void (*)(PagedAttnArgs, PaWork, int);
 
 AttnKernel attn_kernel(int hd, bool e4m3, int G, int* id) {
   static const AttnKernel k[8] = {
@@ -881,13 +1168,16 @@ int attn_ctas(AttnKernel k, int id) {
   return n;
 }
 
+// Rows that share a group's MMA columns.
+int attn_rows(int G) { return G == 1 ? 8 : G == 2 ? 4 : G <= 4 ? 2 : 1; }
+
 }  // namespace
 
 // desc | parts' O | parts' (max, sum), for the largest launch
 size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
   if (T == 0) return 0;
-  const size_t G = nq / nkv;
-  return kPaMaxCtas * (sizeof(int4) + 2 * G * (hd * sizeof(float) + sizeof(float2)));
+  const size_t G = nq / nkv, cols = attn_rows((int)G) * G;
+  return kPaMaxCtas * (sizeof(int4) + 2 * cols * (hd * sizeof(float) + sizeof(float2)));
 }
 
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
@@ -904,17 +1194,21 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
     const long long steps = (segs * row_units + kPaWarps - 1) / kPaWarps;
     if (steps < full) grid = (int)steps;
   }
+  const int rpb = a.req ? attn_rows(G) : 1, cols = rpb * G;
   PaWork ws;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
   ws.desc = reinterpret_cast<int4*>(p);
   ws.o = reinterpret_cast<float*>(p + kPaMaxCtas * sizeof(int4));
-  ws.ml = reinterpret_cast<float2*>(ws.o + (size_t)kPaMaxCtas * 2 * G * a.kv.hd);
-  if (launch_k(k, dim3(grid), dim3(kPaThreads), 0, s, a, ws) != cudaSuccess)
+  ws.ml = reinterpret_cast<float2*>(ws.o + (size_t)kPaMaxCtas * 2 * cols * a.kv.hd);
+  if (launch_k(k, dim3(grid), dim3(kPaThreads), 0, s, a, ws, rpb) != cudaSuccess)
     return SLX_ERR_CUDA;
-  const dim3 jgrid((unsigned)(segs <= grid ? segs : grid), G);
-  auto j = a.kv.hd == 128 ? k_paged_join<128> : k_paged_join<64>;
-  return launch_chained(j, jgrid, dim3(kJoinThreads), 0, s, a, ws) == cudaSuccess
-             ? SLX_OK : SLX_ERR_CUDA;
+  // one CTA per column while they fit the device about twice over
+  const unsigned n = (unsigned)(segs <= grid ? segs : grid);
+  const bool col = n * (unsigned)cols <= 1024;
+  auto j = a.kv.hd == 128 ? (col ? k_paged_join<128, true> : k_paged_join<128, false>)
+                          : (col ? k_paged_join<64, true> : k_paged_join<64, false>);
+  return launch_chained(j, dim3(n, col ? cols : 1), dim3(kJoinThreads), 0, s, a, ws, rpb) ==
+                 cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
 }
 
 }  // namespace slx

@@ -99,16 +99,55 @@ def test_attention_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, E4])
-def test_attention_prompt_rows(dtype):
+@pytest.mark.parametrize("nq,nkv,hd", [(24, 4, 128), (8, 8, 64), (4, 2, 128),
+                                       (9, 3, 64), (12, 1, 64), (1, 1, 128)])
+def test_attention_prompt_rows(nq, nkv, hd, dtype):
     """Several rows of one request (each its own causal length), requests in
     any order, padding rows, the same row twice."""
     lens = [70, 5, 300]
-    host, dev = dev_cache(lens, 4, 128, 16, dtype, seed=4)
-    req = [2] * 20 + [0] * 9 + [-1] + [1] + [0] + [2, 2]
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=4)
+    req = [2] * 20 + [0] * 9 + [-1] + [1] + [0] + [2, 2] + [0, 0, 0, 2]
     pos = [280 + i for i in range(20)] + [61 + i for i in range(9)] + \
-        [-1] + [4] + [0] + [31, 31]
-    out = check_attention(queries(len(req), 24, 128), host, dev, req, pos)
-    assert (out[29] == 0).all()
+        [-1] + [4] + [0] + [31, 31] + [50, -1, 3, 299]
+    out = check_attention(queries(len(req), nq, hd), host, dev, req, pos)
+    assert (out[29] == 0).all() and (out[35] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 8, 64), (4, 2, 128), (12, 4, 128),
+                                       (9, 1, 64)])
+def test_attention_prompt_rows_hide_later_values(nq, nkv, hd, dtype):
+    """Infinite and NaN values of later tokens of a request do not reach the
+    rows before them, and do reach the rows that attend them."""
+    lens = [60, 200]
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=14)
+    pages = host[0].float()
+    for i, n, bad in ((0, 43, float("nan")), (1, 190, float("nan")),
+                      (1, 196, float("nan") if dtype == E4 else float("inf"))):
+        pages[int(host[2][i, n // 16]), 1, :, n % 16] = bad
+    pages = pages.to(dtype)
+    dev = (pages.cuda(), dev[1], dev[2])
+    req = [0] * 16 + [1] * 24
+    pos = list(range(35, 51)) + list(range(176, 200))
+    q = queries(40, nq, hd)
+    out, st = run_attention(q, dev, req, pos)
+    clean = [r for r in range(40) if pos[r] < (43 if req[r] == 0 else 190)]
+    rest = [r for r in range(40) if r not in clean]
+    assert st == 0 and torch.isnan(out[rest]).all()
+    want, bound = P.attention(q[clean], pages, host[1], host[2],
+                              [req[r] for r in clean],
+                              [pos[r] for r in clean], 16, hd ** -0.5)
+    assert ((out[clean].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_long_prompt_rows(dtype):
+    """A chunk of rows behind a long prefix: groups split over CTAs."""
+    lens = [6000, 333]
+    host, dev = dev_cache(lens, 2, 64, 32, dtype, seed=15)
+    req = [0] * 45 + [1] * 6
+    pos = list(range(5955, 6000)) + list(range(327, 333))
+    check_attention(queries(51, 4, 64), host, dev, req, pos)
 
 
 def test_attention_strided_queries():
