@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 import torch
@@ -251,20 +252,21 @@ def lib() -> C.CDLL:
         L.slx_paged_append.restype = i32
         L.slx_paged_append.argtypes = [vp, C.c_int64, i32, i32, vp, vp,
                                        C.c_float, vp, vp, vp,
-                                       C.POINTER(slx_kv_pages), vp, vp, vp]
+                                       vp, vp, vp, vp]
         L.slx_paged_attn_workspace_bytes.restype = sz
         L.slx_paged_attn_workspace_bytes.argtypes = [i32, i32, i32, i32]
         L.slx_paged_attn_decode.restype = i32
         L.slx_paged_attn_decode.argtypes = [vp, C.c_int64, i32, i32,
-                                            C.POINTER(slx_kv_pages), vp, i32,
-                                            i32, vp, vp, C.c_float, vp, vp,
+                                            vp, vp, i32, i32, vp, vp, C.c_float, vp, vp,
                                             sz, vp, vp]
         L.slx_logits_process.restype = i32
-        L.slx_logits_process.argtypes = [vp, i32, i32, i32,
-                                         C.POINTER(slx_logit_rules), vp, vp,
-                                         vp, vp]
+        L.slx_logits_process.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp, vp]
         _lib = L
     return _lib
+
+
+def _fast() -> C.CDLL:
+    return _lib if _lib is not None else lib()
 
 
 def set_pdl(on: bool) -> bool:
@@ -613,74 +615,85 @@ def argmax(logits, out, stream=None) -> None:
     _count(1)
 
 
-def paged_plan(n_new, lengths, lengths_out, table, page_size: int, free_list,
-               n_free, n_free_out, row_req, row_pos, row_slot, row_start,
-               status, stream: int) -> None:
-    """Pages and rows of one step over the requests (stream: raw handle)."""
-    rc = lib().slx_paged_plan(
-        n_new.data_ptr(), lengths.data_ptr(), lengths_out.data_ptr(),
-        table.shape[0], table.data_ptr(), table.shape[1], page_size,
-        free_list.data_ptr(), free_list.shape[0], n_free.data_ptr(),
-        n_free_out.data_ptr(), row_req.data_ptr(), row_pos.data_ptr(),
-        row_slot.data_ptr(), row_req.shape[0], row_start.data_ptr(),
-        status.data_ptr(), stream)
-    _check("slx_paged_plan", rc)
-    _count(1)
+# Batched decode (slx_paged_*, slx_logits_process).  These wrappers run once
+# per layer or step of a server's loop: they take addresses and sizes that
+# ops.py has checked, and the argument structs as packed bytes.
+_KV_PAGES = struct.Struct("@PPPiiiii")
+_LOGIT_RULES = struct.Struct("@10Piii")
+assert _KV_PAGES.size <= C.sizeof(slx_kv_pages)
+assert _LOGIT_RULES.size <= C.sizeof(slx_logit_rules)
 
 
-def kv_pages(pages: torch.Tensor, kv_scale) -> slx_kv_pages:
-    """pages [n_pages, 2, n_kv, page_size, head_dim]; kv_scale [2, n_kv]
-    fp32 (e4m3 pages) or None."""
-    n, _, n_kv, ps, hd = pages.shape
-    if kv_scale is None:
-        return slx_kv_pages(pages.data_ptr(), None, None, n, ps, n_kv, hd,
-                            KV_BF16)
-    k = kv_scale.data_ptr()
-    return slx_kv_pages(pages.data_ptr(), k, k + 4 * n_kv, n, ps, n_kv, hd,
-                        KV_E4M3)
+def kv_pages(base: int, kv_scale: int, n_pages: int, n_kv: int,
+             page_size: int, head_dim: int) -> bytes:
+    """slx_kv_pages of pages at `base` (kv_scale: fp32 [2, n_kv] of e4m3
+    pages, 0 for bf16)."""
+    return _KV_PAGES.pack(base, kv_scale, kv_scale and kv_scale + 4 * n_kv,
+                          n_pages, page_size, n_kv, head_dim,
+                          KV_E4M3 if kv_scale else KV_BF16) + _PAD
 
 
-def paged_append(qkv, pages: slx_kv_pages, slot, pos, n_q: int, q_norm,
-                 k_norm, eps: float, inv_freq, q_out, status,
-                 stream: int) -> None:
+def logit_rules(*fields: int) -> bytes:
+    """slx_logit_rules, fields in the header's order (0: not given)."""
+    return _LOGIT_RULES.pack(*fields) + _PAD
+
+
+_PAD = bytes(8)             # the structs' tail padding
+
+
+def paged_plan(n_new: int, lengths: int, lengths_out: int, n_req: int,
+               table: int, max_pages: int, page_size: int, free_list: int,
+               n_pages: int, n_free: int, n_free_out: int, rows: int,
+               n_rows: int, row_start: int, status: int, stream: int) -> None:
+    """Pages and rows of one step (rows: request, position, slot, one after
+    the other)."""
+    rc = _fast().slx_paged_plan(
+        n_new, lengths, lengths_out, n_req, table, max_pages, page_size,
+        free_list, n_pages, n_free, n_free_out, rows, rows + 4 * n_rows,
+        rows + 8 * n_rows, n_rows, row_start, status, stream)
+    if rc:
+        _check("slx_paged_plan", rc)
+    LAUNCHES[0] += 1
+
+
+def paged_append(qkv: int, stride: int, T: int, n_q: int, q_norm: int,
+                 k_norm: int, eps: float, inv_freq: int, pos: int, slot: int,
+                 pages: bytes, q_out: int, status: int, stream: int) -> None:
     """q/k norm + RoPE, queries to q_out, keys and values to the pages."""
-    rc = lib().slx_paged_append(
-        qkv.data_ptr(), qkv.stride(0), qkv.shape[0], n_q, q_norm.data_ptr(),
-        k_norm.data_ptr(), eps, inv_freq.data_ptr(), pos.data_ptr(),
-        slot.data_ptr(), C.byref(pages), q_out.data_ptr(), status.data_ptr(),
-        stream)
-    _check("slx_paged_append", rc)
-    _count(1)
+    rc = _fast().slx_paged_append(qkv, stride, T, n_q, q_norm, k_norm, eps,
+                                  inv_freq, pos, slot, pages, q_out, status,
+                                  stream)
+    if rc:
+        _check("slx_paged_append", rc)
+    LAUNCHES[0] += 1
 
 
 def paged_attn_workspace_bytes(T: int, n_q: int, n_kv: int,
                                head_dim: int) -> int:
-    return int(lib().slx_paged_attn_workspace_bytes(T, n_q, n_kv, head_dim))
+    return _fast().slx_paged_attn_workspace_bytes(T, n_q, n_kv, head_dim)
 
 
-def paged_attn_decode(q, q_stride: int, n_q: int, pages: slx_kv_pages, table,
-                      req, pos, scale: float, out, workspace, status,
-                      stream: int) -> None:
-    """Attention of pos.shape[0] rows over the pages."""
-    rc = lib().slx_paged_attn_decode(
-        q.data_ptr(), q_stride, pos.shape[0], n_q, C.byref(pages),
-        table.data_ptr(), table.shape[0], table.shape[1], ptr(req),
-        pos.data_ptr(), scale, out.data_ptr(), ptr(workspace),
-        0 if workspace is None else workspace.shape[0], status.data_ptr(),
-        stream)
-    _check("slx_paged_attn_decode", rc)
-    _count(1)
+def paged_attn_decode(q: int, q_stride: int, T: int, n_q: int, pages: bytes,
+                      table: int, n_req: int, max_pages: int, req, pos: int,
+                      scale: float, out: int, workspace: int, nbytes: int,
+                      status: int, stream: int) -> None:
+    """Attention of T rows over the pages (two launches)."""
+    rc = _fast().slx_paged_attn_decode(q, q_stride, T, n_q, pages, table,
+                                       n_req, max_pages, req, pos, scale, out,
+                                       workspace, nbytes, status, stream)
+    if rc:
+        _check("slx_paged_attn_decode", rc)
+    LAUNCHES[0] += 2
 
 
-def logits_process(logits, rules: slx_logit_rules, out, pick, status,
-                   stream: int) -> None:
+def logits_process(logits: int, f32: bool, T: int, V: int, rules: bytes, out,
+                   pick: int, status: int, stream: int) -> None:
     """Penalties, biases, mask and greedy pick of logits [T, V]."""
-    rc = lib().slx_logits_process(
-        logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0,
-        logits.shape[0], logits.shape[1], C.byref(rules), ptr(out), ptr(pick),
-        status.data_ptr(), stream)
-    _check("slx_logits_process", rc)
-    _count(1)
+    rc = _fast().slx_logits_process(logits, f32, T, V, rules, out, pick,
+                                    status, stream)
+    if rc:
+        _check("slx_logits_process", rc)
+    LAUNCHES[0] += 1
 
 
 def pread_many(fds: np.ndarray, offsets: np.ndarray, sizes: np.ndarray,

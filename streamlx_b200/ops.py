@@ -219,60 +219,63 @@ class PagedPlan(NamedTuple):
     n_free: torch.Tensor    # [1] free pages after it
 
 
+_I32, _F32 = torch.int32, torch.float32
+_BF16, _E4M3 = torch.bfloat16, torch.float8_e4m3fn
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_cur_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
-def _ints(t, n: int, device, name: str) -> None:
-    if (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or
-            t.device != device or not t.is_contiguous()):
-        raise ValueError(f"{name}: contiguous int32 [{n}] on {device} wanted, "
-                         f"got {t.dtype} {list(t.shape)} on {t.device}")
-
-
-def _floats(t, n: int, device, name: str) -> None:
-    if (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or
-            t.device != device or not t.is_contiguous()):
-        raise ValueError(f"{name}: contiguous float32 [{n}] on {device} "
+def _vec(t, n: int, dtype, idx: int, name: str) -> int:
+    """Address of a contiguous vector [n] of a type on device idx."""
+    if (t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or
+            t.get_device() != idx or not t.is_contiguous()):
+        raise ValueError(f"{name}: contiguous {dtype} [{n}] on cuda:{idx} "
                          f"wanted, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
-def _raw_stream(device) -> int:
-    """Current stream of a device, as the C ABI takes it."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _call_status(status, idx: int) -> int:
+    """Address of the call's status word: the given one, else the device's.
+    A capture that comes before the device's first call has none unless it is
+    given one (a word born in a graph's memory would be cleared by every
+    replay): its device errors are not reported."""
+    if status is not None:
+        return _vec(status, 1, _I32, idx, "status")
+    dev = torch.device("cuda", idx)
+    t = _scratch.get(("status", dev))
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        t = _status(dev)
+    return t.data_ptr()
 
 
-def _call_status(device) -> torch.Tensor:
-    """The device's status word; inside a capture that comes before its
-    first use, one of the graph's own (the shared word must not be born in a
-    graph's memory, where every replay would clear it)."""
-    t = _scratch.get(("status", device))
-    if t is not None:
-        return t
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(1, dtype=torch.int32, device=device)
-    return _status(device)
-
-
-def _pages_of(pages: torch.Tensor, kv_scale, name: str) -> "L.slx_kv_pages":
-    _need(pages.is_cuda and pages.dim() == 5 and pages.shape[1] == 2 and
-          pages.is_contiguous(),
-          f"{name}: pages must be contiguous [n_pages, 2, n_kv, page_size, "
-          "head_dim] on a CUDA device")
-    if pages.dtype == torch.bfloat16:
+def _pages_of(pages: torch.Tensor, kv_scale, name: str):
+    """(slx_kv_pages as bytes, n_kv, head_dim) of a layer's pages."""
+    shape = pages.shape
+    if (len(shape) != 5 or shape[1] != 2 or not pages.is_cuda or
+            not pages.is_contiguous()):
+        raise ValueError(f"{name}: pages must be contiguous [n_pages, 2, n_kv, "
+                         "page_size, head_dim] on a CUDA device")
+    n, _, n_kv, ps, hd = shape
+    if pages.dtype is _BF16:
         _need(kv_scale is None, f"{name}: bf16 pages take no kv_scale")
-    elif pages.dtype == torch.float8_e4m3fn:
-        n_kv = pages.shape[2]
-        _need(kv_scale is not None and kv_scale.dtype == torch.float32 and
-              list(kv_scale.shape) == [2, n_kv] and
-              kv_scale.device == pages.device and kv_scale.is_contiguous(),
-              f"{name}: e4m3 pages need kv_scale, float32 [2, {n_kv}] (keys, "
-              "values) on their device")
-    else:
+        return L.kv_pages(pages.data_ptr(), 0, n, n_kv, ps, hd), n_kv, hd
+    if pages.dtype is not _E4M3:
         raise ValueError(f"{name}: pages are bfloat16 or float8_e4m3fn, got "
                          f"{pages.dtype}")
-    return L.kv_pages(pages, kv_scale)
+    if (kv_scale is None or kv_scale.dtype is not _F32 or
+            kv_scale.shape != (2, n_kv) or not kv_scale.is_contiguous() or
+            kv_scale.get_device() != pages.get_device()):
+        raise ValueError(f"{name}: e4m3 pages need kv_scale, float32 [2, {n_kv}]"
+                         " (keys, values) on their device")
+    return (L.kv_pages(pages.data_ptr(), kv_scale.data_ptr(), n, n_kv, ps, hd),
+            n_kv, hd)
 
 
 def paged_plan(n_new: torch.Tensor, lengths: torch.Tensor,
@@ -288,38 +291,37 @@ def paged_plan(n_new: torch.Tensor, lengths: torch.Tensor,
     updated; ``lengths_out`` / ``n_free_out`` may be ``lengths`` /
     ``n_free`` themselves.  When pages or rows do not suffice nothing
     changes, every row is padding and the status word says SLX_ERR_PAGES."""
-    dev = table.device
-    _need(table.is_cuda and table.dim() == 2 and table.dtype == torch.int32
-          and table.is_contiguous(),
-          "paged_plan: table must be contiguous int32 [n_req, max_pages] on a "
-          "CUDA device")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    if (not table.is_cuda or table.dim() != 2 or table.dtype is not _I32 or
+            not table.is_contiguous()):
+        raise ValueError("paged_plan: table must be contiguous int32 [n_req, "
+                         "max_pages] on a CUDA device")
+    idx = table.get_device()
+    if idx != _cur_device():
+        with torch.cuda.device(idx):
             return paged_plan(n_new, lengths, table, free_list, n_free,
                               page_size, n_rows, lengths_out=lengths_out,
                               n_free_out=n_free_out, status=status)
-    R = table.shape[0]
-    _need(page_size in PAGE_SIZES, f"paged_plan: page_size {page_size}")
+    R, max_pages = table.shape
+    n_pages = free_list.numel()
     _need(n_rows >= 0, f"paged_plan: n_rows {n_rows}")
-    _ints(n_new, R, dev, "paged_plan: n_new")
-    _ints(lengths, R, dev, "paged_plan: lengths")
-    _ints(free_list, free_list.numel(), dev, "paged_plan: free_list")
-    _ints(n_free, 1, dev, "paged_plan: n_free")
-    rows = torch.empty(3, n_rows, dtype=torch.int32, device=dev)
-    start = torch.empty(R + 1, dtype=torch.int32, device=dev)
+    # rows (request, position, slot), their starts and the state after the
+    # step, one allocation
+    buf = torch.empty(3 * n_rows + 2 * R + 2, dtype=_I32, device=table.device)
+    req, pos, slot, start, ln, nf = buf.split(
+        (n_rows, n_rows, n_rows, R + 1, R, 1))
     if lengths_out is None:
-        lengths_out = torch.empty_like(lengths)
-    else:
-        _ints(lengths_out, R, dev, "paged_plan: lengths_out")
+        lengths_out = ln
     if n_free_out is None:
-        n_free_out = torch.empty_like(n_free)
-    else:
-        _ints(n_free_out, 1, dev, "paged_plan: n_free_out")
-    req, pos, slot = rows.unbind(0)
-    L.paged_plan(n_new, lengths, lengths_out, table, page_size, free_list,
-                 n_free, n_free_out, req, pos, slot, start,
-                 _call_status(dev) if status is None else status,
-                 _raw_stream(dev))
+        n_free_out = nf
+    L.paged_plan(_vec(n_new, R, _I32, idx, "paged_plan: n_new"),
+                 _vec(lengths, R, _I32, idx, "paged_plan: lengths"),
+                 _vec(lengths_out, R, _I32, idx, "paged_plan: lengths_out"),
+                 R, table.data_ptr(), max_pages, page_size,
+                 _vec(free_list, n_pages, _I32, idx, "paged_plan: free_list"),
+                 n_pages, _vec(n_free, 1, _I32, idx, "paged_plan: n_free"),
+                 _vec(n_free_out, 1, _I32, idx, "paged_plan: n_free_out"),
+                 buf.data_ptr(), n_rows, start.data_ptr(),
+                 _call_status(status, idx), _raw_stream(idx))
     return PagedPlan(req, pos, slot, start, lengths_out, n_free_out)
 
 
@@ -333,37 +335,33 @@ def paged_append(qkv: torch.Tensor, pages: torch.Tensor, slot: torch.Tensor,
     qkv [T, (n_q + 2 n_kv) * head_dim] bf16 (rows may be strided); returns
     the rotated queries [T, n_q, head_dim].  Rows with slot or pos < 0 give
     zero queries and write no page."""
-    dev = pages.device
-    kv = _pages_of(pages, kv_scale, "paged_append")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    kv, n_kv, hd = _pages_of(pages, kv_scale, "paged_append")
+    idx = pages.get_device()
+    if idx != _cur_device():
+        with torch.cuda.device(idx):
             return paged_append(qkv, pages, slot, pos, n_q, q_norm, k_norm,
                                 eps, inv_freq, kv_scale=kv_scale, q_out=q_out,
                                 status=status)
-    T, hd = qkv.shape[0], pages.shape[4]
-    _need(qkv.dtype == torch.bfloat16 and qkv.dim() == 2 and
-          qkv.device == dev and
-          qkv.shape[1] == (n_q + 2 * pages.shape[2]) * hd and
-          qkv.stride(1) == 1,
-          "paged_append: qkv must be bfloat16 [T, (n_q + 2 n_kv) * head_dim] "
-          "on the pages' device")
-    _ints(slot, T, dev, "paged_append: slot")
-    _ints(pos, T, dev, "paged_append: pos")
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _need(w.dtype == torch.bfloat16 and w.numel() == hd and
-              w.device == dev and w.is_contiguous(),
-              f"paged_append: {name} must be bfloat16 [{hd}]")
-    _floats(inv_freq, hd // 2, dev, "paged_append: inv_freq")
+    if (qkv.dtype is not _BF16 or qkv.dim() != 2 or qkv.get_device() != idx or
+            qkv.shape[1] != (n_q + 2 * n_kv) * hd or qkv.stride(1) != 1):
+        raise ValueError("paged_append: qkv must be bfloat16 [T, (n_q + 2 n_kv)"
+                         " * head_dim] on the pages' device")
+    T = qkv.shape[0]
     if q_out is None:
-        q_out = torch.empty(T, n_q, hd, dtype=torch.bfloat16, device=dev)
-    else:
-        _need(q_out.dtype == torch.bfloat16 and q_out.device == dev and
-              q_out.numel() == T * n_q * hd and q_out.is_contiguous(),
-              "paged_append: q_out must be contiguous bfloat16 [T, n_q, "
-              "head_dim]")
-    L.paged_append(qkv, kv, slot, pos, n_q, q_norm, k_norm, eps, inv_freq,
-                   q_out, _call_status(dev) if status is None else status,
-                   _raw_stream(dev))
+        q_out = qkv.new_empty((T, n_q, hd))
+    elif (q_out.dtype is not _BF16 or q_out.get_device() != idx or
+          q_out.numel() != T * n_q * hd or not q_out.is_contiguous()):
+        raise ValueError("paged_append: q_out must be contiguous bfloat16 [T, "
+                         "n_q, head_dim]")
+    L.paged_append(qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], T,
+                   n_q, _vec(q_norm, hd, _BF16, idx, "paged_append: q_norm"),
+                   _vec(k_norm, hd, _BF16, idx, "paged_append: k_norm"), eps,
+                   _vec(inv_freq, hd // 2, _F32, idx,
+                        "paged_append: inv_freq"),
+                   _vec(pos, T, _I32, idx, "paged_append: pos"),
+                   _vec(slot, T, _I32, idx, "paged_append: slot"), kv,
+                   q_out.data_ptr(), _call_status(status, idx),
+                   _raw_stream(idx))
     return q_out
 
 
@@ -388,47 +386,49 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor,
     (``slx_paged_attn_decode``): row t of q [T, n_q, head_dim] (rows may be
     strided) attends positions 0..pos[t] of request req[t] (default: t);
     pos[t] < 0 gives zeros.  Returns [T, n_q, head_dim] bf16."""
-    dev = pages.device
-    kv = _pages_of(pages, kv_scale, "paged_attention")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    kv, n_kv, hd = _pages_of(pages, kv_scale, "paged_attention")
+    idx = pages.get_device()
+    if idx != _cur_device():
+        with torch.cuda.device(idx):
             return paged_attention(q, pages, table, pos, req=req, scale=scale,
                                    kv_scale=kv_scale, out=out,
                                    workspace=workspace, status=status)
-    hd = pages.shape[4]
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.device == dev and
-          q.shape[2] == hd and q.stride(2) == 1 and
-          (q.stride(1) == hd or q.shape[1] == 1),
-          "paged_attention: q must be bfloat16 [T, n_q, head_dim] with "
-          "adjacent heads, on the pages' device")
-    T, n_q = q.shape[0], q.shape[1]
-    _need(table.dim() == 2 and table.dtype == torch.int32 and
-          table.device == dev and table.is_contiguous(),
-          "paged_attention: table must be contiguous int32 [n_req, max_pages]")
-    _ints(pos, T, dev, "paged_attention: pos")
-    if req is not None:
-        _ints(req, T, dev, "paged_attention: req")
-    if scale is None:
-        scale = hd ** -0.5
+    shape, stride = q.shape, q.stride()
+    if (len(shape) != 3 or q.dtype is not _BF16 or q.get_device() != idx or
+            shape[2] != hd or stride[2] != 1 or
+            (stride[1] != hd and shape[1] != 1)):
+        raise ValueError("paged_attention: q must be bfloat16 [T, n_q, "
+                         "head_dim] with adjacent heads, on the pages' device")
+    T, n_q, _ = shape
+    if (table.dim() != 2 or table.dtype is not _I32 or
+            table.get_device() != idx or not table.is_contiguous()):
+        raise ValueError("paged_attention: table must be contiguous int32 "
+                         "[n_req, max_pages]")
+    n_req, max_pages = table.shape
     if out is None:
-        out = torch.empty(T, n_q, hd, dtype=torch.bfloat16, device=dev)
-    else:
-        _need(out.dtype == torch.bfloat16 and out.device == dev and
-              out.numel() == T * n_q * hd and out.is_contiguous(),
-              "paged_attention: out must be contiguous bfloat16 [T, n_q, "
-              "head_dim]")
+        out = q.new_empty(shape)
+    elif (out.dtype is not _BF16 or out.get_device() != idx or
+          out.numel() != T * n_q * hd or not out.is_contiguous()):
+        raise ValueError("paged_attention: out must be contiguous bfloat16 [T, "
+                         "n_q, head_dim]")
     if workspace is None:
         # the call's own: calls on other streams or in graphs share nothing
-        workspace = paged_workspace(T, n_q, pages.shape[2], hd, dev)
-    else:
-        _need(workspace.dtype == torch.uint8 and workspace.dim() == 1 and
-              workspace.device == dev and workspace.is_contiguous(),
-              "paged_attention: workspace must come from paged_workspace on "
-              "the pages' device")
-    L.paged_attn_decode(q, q.stride(0) if T > 1 else n_q * hd, n_q, kv, table,
-                        req, pos, scale, out, workspace,
-                        _call_status(dev) if status is None else status,
-                        _raw_stream(dev))
+        workspace = q.new_empty(
+            max(L.paged_attn_workspace_bytes(T, n_q, n_kv, hd), 16),
+            dtype=torch.uint8)
+    elif (workspace.dtype is not torch.uint8 or workspace.dim() != 1 or
+          workspace.get_device() != idx or not workspace.is_contiguous()):
+        raise ValueError("paged_attention: workspace must come from "
+                         "paged_workspace on the pages' device")
+    L.paged_attn_decode(
+        q.data_ptr(), stride[0] if T > 1 else n_q * hd, T, n_q, kv,
+        table.data_ptr(), n_req, max_pages,
+        None if req is None else _vec(req, T, _I32, idx,
+                                      "paged_attention: req"),
+        _vec(pos, T, _I32, idx, "paged_attention: pos"),
+        hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        workspace.data_ptr(), workspace.shape[0], _call_status(status, idx),
+        _raw_stream(idx))
     return out
 
 
@@ -455,13 +455,14 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     None computes the pick alone.  Returns the picks (int32 [T], -1 where the
     mask allows nothing), written to ``pick`` if that is a tensor; None with
     ``pick=False``."""
-    dev = logits.device
-    _need(logits.is_cuda and logits.dim() == 2 and logits.is_contiguous() and
-          logits.dtype in (torch.bfloat16, torch.float32),
-          "process_logits: logits must be contiguous bfloat16 or float32 "
-          "[T, V] on a CUDA device")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    if (not logits.is_cuda or logits.dim() != 2 or
+            not logits.is_contiguous() or
+            logits.dtype not in (_BF16, _F32)):
+        raise ValueError("process_logits: logits must be contiguous bfloat16 "
+                         "or float32 [T, V] on a CUDA device")
+    idx = logits.get_device()
+    if idx != _cur_device():
+        with torch.cuda.device(idx):
             return process_logits(logits, history, n_prompt, n_history,
                                   repetition=repetition, frequency=frequency,
                                   presence=presence, bias=bias, mask=mask,
@@ -469,64 +470,62 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     T, V = logits.shape
     _need(pick is not False or out is not None,
           "process_logits: neither out nor pick wanted")
-    r = L.slx_logit_rules()
+
+    def vec(t, n, dtype, name):
+        return 0 if t is None else _vec(t, n, dtype, idx,
+                                        "process_logits: " + name)
+
+    hist = stride = n_h = n_p = rep = freq = pres = 0
     if history is not None:
-        _need(history.dtype == torch.int32 and history.dim() == 2 and
-              history.shape[0] == T and history.device == dev and
-              history.is_contiguous() and n_history is not None,
-              "process_logits: history must be contiguous int32 [T, max] "
-              "with n_history")
-        _ints(n_history, T, dev, "process_logits: n_history")
-        if history.shape[1] > 0:
-            r.history = history.data_ptr()
-            r.history_stride = history.shape[1]
-            r.n_history = n_history.data_ptr()
-            if n_prompt is not None:
-                _ints(n_prompt, T, dev, "process_logits: n_prompt")
-                r.n_prompt = n_prompt.data_ptr()
-            if repetition is not None:
-                _floats(repetition, T, dev, "process_logits: repetition")
-                r.repetition = repetition.data_ptr()
-            if frequency is not None:
-                _floats(frequency, T, dev, "process_logits: frequency")
-                r.frequency = frequency.data_ptr()
-            if presence is not None:
-                _floats(presence, T, dev, "process_logits: presence")
-                r.presence = presence.data_ptr()
+        if (history.dtype is not _I32 or history.dim() != 2 or
+                history.shape[0] != T or history.get_device() != idx or
+                not history.is_contiguous() or n_history is None):
+            raise ValueError("process_logits: history must be contiguous int32 "
+                             "[T, max] with n_history")
+        n_h = vec(n_history, T, _I32, "n_history")
+        n_p = vec(n_prompt, T, _I32, "n_prompt")
+        rep = vec(repetition, T, _F32, "repetition")
+        freq = vec(frequency, T, _F32, "frequency")
+        pres = vec(presence, T, _F32, "presence")
+        stride = history.shape[1]
+        if stride > 0:
+            hist = history.data_ptr()
+        else:                       # nothing to count
+            n_h = n_p = rep = freq = pres = 0
     else:
         _need(repetition is None and frequency is None and presence is None
               and n_prompt is None and n_history is None,
               "process_logits: penalties need a history")
+    b_ids = b_vals = b_start = n_bias = 0
     if bias is not None:
         ids, vals, start = bias
-        n = ids.numel()
-        _ints(ids, n, dev, "process_logits: bias ids")
-        _floats(vals, n, dev, "process_logits: bias values")
-        _ints(start, T + 1, dev, "process_logits: bias start")
-        if n > 0:
-            r.bias_ids = ids.data_ptr()
-            r.bias_values = vals.data_ptr()
-            r.bias_start = start.data_ptr()
-            r.n_bias = n
+        n_bias = ids.numel()
+        b_ids = vec(ids, n_bias, _I32, "bias ids")
+        b_vals = vec(vals, n_bias, _F32, "bias values")
+        b_start = vec(start, T + 1, _I32, "bias start")
+        if n_bias == 0:
+            b_ids = b_vals = b_start = 0
+    m = m_stride = 0
     if mask is not None:
-        _need(mask.dtype == torch.int32 and mask.dim() == 2 and
-              mask.shape[0] == T and mask.shape[1] >= (V + 31) // 32 and
-              mask.device == dev and mask.is_contiguous(),
-              "process_logits: mask must be contiguous int32 [T, >= "
-              "ceil(V / 32)]")
-        r.mask = mask.data_ptr()
-        r.mask_stride = mask.shape[1]
-    if out is not None:
-        _need(out.dtype == logits.dtype and out.shape == logits.shape and
-              out.device == dev and out.is_contiguous(),
-              "process_logits: out must match logits")
+        if (mask.dtype is not _I32 or mask.dim() != 2 or mask.shape[0] != T or
+                mask.shape[1] * 32 < V or mask.get_device() != idx or
+                not mask.is_contiguous()):
+            raise ValueError("process_logits: mask must be contiguous int32 "
+                             "[T, >= ceil(V / 32)]")
+        m, m_stride = mask.data_ptr(), mask.shape[1]
+    if out is not None and (out.dtype is not logits.dtype or
+                            out.shape != logits.shape or
+                            out.get_device() != idx or
+                            not out.is_contiguous()):
+        raise ValueError("process_logits: out must match logits")
     if pick is None:
-        pick = torch.empty(T, dtype=torch.int32, device=dev)
+        pick = logits.new_empty(T, dtype=_I32)
     elif pick is False:
         pick = None
-    else:
-        _ints(pick, T, dev, "process_logits: pick")
-    L.logits_process(logits, r, out, pick,
-                     _call_status(dev) if status is None else status,
-                     _raw_stream(dev))
+    L.logits_process(
+        logits.data_ptr(), logits.dtype is _F32, T, V,
+        L.logit_rules(hist, n_p, n_h, rep, freq, pres, b_ids, b_vals, b_start,
+                      m, stride, n_bias, m_stride),
+        None if out is None else out.data_ptr(), vec(pick, T, _I32, "pick"),
+        _call_status(status, idx), _raw_stream(idx))
     return pick
