@@ -200,6 +200,28 @@ cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block,
   return launch_attr(pdl_enabled(), kernel, grid, block, smem, stream, args...);
 }
 
+// launch_k with clusters of `ctas` CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(int ctas, void (*kernel)(KArgs...), dim3 grid,
+                           dim3 block, size_t smem, cudaStream_t stream,
+                           Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 // The second launch of one call, as a PDL secondary of the first whatever
 // the caller's setting.
 template <typename... KArgs, typename... Args>

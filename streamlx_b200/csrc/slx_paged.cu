@@ -15,6 +15,7 @@ namespace cg = cooperative_groups;
 // ------------------------------------------------------------------ plan --
 
 constexpr int kPlanThreads = 512;
+constexpr int kPlanCluster = 8;
 
 // Largest i with s[i] <= v (s ascending, s[0] = 0 <= v < s[n]): the request
 // an item belongs to, requests without items being skipped.
@@ -39,7 +40,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
   int32_t* s_get = s_row + a.n_req + 1;     // [n_req + 1]
   int32_t* s_back = s_get + a.n_req + 1;    // [n_req + 1]
   int32_t* s_len = s_back + a.n_req + 1;    // [n_req]
-  __shared__ long long w_sum[3][kPlanThreads / 32];
+  __shared__ __align__(16) int w_sum[3][kPlanThreads / 32];
   __shared__ int s_bad;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -49,77 +50,75 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
   pdl_wait_primary();
   if (tid == 0) s_bad = 0;
   __syncthreads();
+  const int n_free = *a.n_free;
   const int per = (a.n_req + kPlanThreads - 1) / kPlanThreads;
   const int r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
-  auto pages = [&](long long n) { return (n + a.page_size - 1) >> sh; };
-  // counts of request i; false when its numbers are out of range
-  auto counts = [&](int i, long long (&c)[3], int& len) {
-    const int nw = a.n_new[i];
-    len = a.lengths[i];
-    c[0] = c[1] = c[2] = 0;
-    if (nw < -1 || len < 0 || len + (long long)max(nw, 0) > cap) return false;
-    if (nw < 0) {
+  auto pages = [&](long long n) { return (int)((n + a.page_size - 1) >> sh); };
+  // sums stop at 2^31 - 1: more rows or pages than any step can have
+  auto add = [](int x, int y) { return (int)min((unsigned)x + (unsigned)y, 0x7fffffffu); };
+  int sum[3] = {0, 0, 0};
+  for (int i = r0; i < r1; ++i) {
+    const int nw = a.n_new[i], len = a.lengths[i];
+    int c[3] = {0, 0, 0};
+    if (nw < -1 || len < 0 || len + (long long)max(nw, 0) > cap) {
+      s_bad = 1;
+    } else if (nw < 0) {
       c[2] = pages(len);
     } else {
       c[0] = nw;
       c[1] = pages((long long)len + nw) - pages(len);
     }
-    return true;
-  };
-  long long sum[3] = {0, 0, 0};
-  for (int i = r0; i < r1; ++i) {
-    long long c[3];
-    int len;
-    if (!counts(i, c, len)) s_bad = 1;
     s_len[i] = len;
+    s_row[i] = c[0];
+    s_get[i] = c[1];
+    s_back[i] = c[2];
 #pragma unroll
-    for (int q = 0; q < 3; ++q) sum[q] += c[q];
+    for (int q = 0; q < 3; ++q) sum[q] = add(sum[q], c[q]);
   }
-  long long inc[3];
+  int inc[3];
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
-    long long v = sum[q];
+    int v = sum[q];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = add(v, u);
     }
     inc[q] = v;
     if (lane == 31) w_sum[q][warp] = v;
   }
-  const int n_free = *a.n_free;
   __syncthreads();
-  long long tot[3], at[3];
+  int tot[3], at[3];
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
-    long long before = 0, all = 0;
+    int before = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < kPlanThreads / 32; ++w) {
-      if (w < warp) before += w_sum[q][w];
-      all += w_sum[q][w];
+      if (w == warp) before = all;
+      all = add(all, w_sum[q][w]);
     }
     tot[q] = all;
-    at[q] = before + inc[q] - sum[q];
+    at[q] = add(before, inc[q]) - sum[q];
   }
   int code = SLX_OK;
-  if (s_bad || n_free < 0 || n_free + tot[2] > a.n_pages)
+  if (s_bad || n_free < 0 || n_free > a.n_pages || tot[2] > a.n_pages - n_free)
     code = SLX_ERR_OUT_OF_RANGE;
   else if (tot[0] > a.n_rows || tot[1] > n_free + tot[2])
     code = SLX_ERR_PAGES;
   if (code == SLX_OK) {
     for (int i = r0; i < r1; ++i) {
-      long long c[3];
-      int len;
-      counts(i, c, len);
-      s_row[i] = (int)at[0];
-      s_get[i] = (int)at[1];
-      s_back[i] = (int)at[2];
+      int32_t* const pre[3] = {s_row, s_get, s_back};
 #pragma unroll
-      for (int q = 0; q < 3; ++q) at[q] += c[q];
+      for (int q = 0; q < 3; ++q) {
+        const int c = pre[q][i];
+        pre[q][i] = at[q];
+        at[q] += c;
+      }
     }
     if (tid == 0) {
-      s_row[a.n_req] = (int)tot[0];
-      s_get[a.n_req] = (int)tot[1];
-      s_back[a.n_req] = (int)tot[2];
+      s_row[a.n_req] = tot[0];
+      s_get[a.n_req] = tot[1];
+      s_back[a.n_req] = tot[2];
     }
   }
   cluster.sync();  // every CTA has read lengths and n_free
@@ -138,7 +137,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
       a.row_req[r] = a.row_pos[r] = a.row_slot[r] = -1;
     return;
   }
-  const int n_back = (int)tot[2], n_get = (int)tot[1], n_rows = (int)tot[0];
+  const int n_back = tot[2], n_get = tot[1], n_rows = tot[0];
   const int top = n_free + n_back;
   for (int g = gt; g < n_back; g += gn) {
     const int i = owner_of(s_back, a.n_req, g);
@@ -151,33 +150,51 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
   }
   if (gt == 0) *a.n_free_out = top - n_get;
   cluster.sync();  // the pushed pages are on the stack
-  // the page that is the g-th to be popped
-  auto popped = [&](int g) {
-    const int p = __ldcg(a.free_list + (top - 1 - g));
-    if (p < 0 || p >= a.n_pages) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
-    return p;
-  };
-  for (int g = gt; g < n_get; g += gn) {
-    const int i = owner_of(s_get, a.n_req, g);
-    const int had = (int)pages(s_len[i]);
-    a.table[(size_t)i * a.max_pages + had + (g - s_get[i])] = popped(g);
-  }
-  for (int r = gt; r < a.n_rows; r += gn) {
-    int req = -1, pos = -1, slot = -1;
-    if (r < n_rows) {
-      req = owner_of(s_row, a.n_req, r);
-      pos = s_len[req] + (r - s_row[req]);
-      const int col = pos >> sh, had = (int)pages(s_len[req]);
-      const int p = col < had ? a.table[(size_t)req * a.max_pages + col]
-                              : popped(s_get[req] + (col - had));
-      if (p < 0 || p >= a.n_pages)
-        set_status(a.status, SLX_ERR_OUT_OF_RANGE);
-      else
-        slot = (p << sh) + (pos & (a.page_size - 1));
+  // four items at a time: their reads of the stack and the table overlap
+  constexpr int B = 4;
+  for (int g0 = gt; g0 < n_get; g0 += B * gn) {
+    int p[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      p[j] = g0 + j * gn < n_get ? __ldcg(a.free_list + (top - 1 - (g0 + j * gn))) : 0;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int g = g0 + j * gn;
+      if (g >= n_get) break;
+      const int i = owner_of(s_get, a.n_req, g);
+      if (p[j] < 0 || p[j] >= a.n_pages) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+      a.table[(size_t)i * a.max_pages + pages(s_len[i]) + (g - s_get[i])] = p[j];
     }
-    a.row_req[r] = req;
-    a.row_pos[r] = pos;
-    a.row_slot[r] = slot;
+  }
+  for (int t0 = gt; t0 < a.n_rows; t0 += B * gn) {
+    int req[B], pos[B], p[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int r = t0 + j * gn;
+      req[j] = pos[j] = p[j] = -1;
+      if (r < n_rows) {
+        const int i = owner_of(s_row, a.n_req, r);
+        req[j] = i;
+        pos[j] = s_len[i] + (r - s_row[i]);
+        const int col = pos[j] >> sh, had = pages(s_len[i]);
+        // an old page from the table, a new one as it was popped
+        p[j] = col < had ? a.table[(size_t)i * a.max_pages + col]
+                         : __ldcg(a.free_list + (top - 1 - (s_get[i] + (col - had))));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int r = t0 + j * gn;
+      if (r >= a.n_rows) break;
+      int slot = -1;
+      if (p[j] >= 0 && p[j] < a.n_pages)
+        slot = (p[j] << sh) + (pos[j] & (a.page_size - 1));
+      else if (r < n_rows)
+        set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+      a.row_req[r] = req[j];
+      a.row_pos[r] = pos[j];
+      a.row_slot[r] = slot;
+    }
   }
 }
 
@@ -191,113 +208,179 @@ int launch_paged_plan(const PlanArgs& a, cudaStream_t s) {
       return SLX_ERR_CUDA;
     slot.store(1, std::memory_order_relaxed);
   }
-  return launch_k(k_paged_plan, dim3(1), dim3(kPlanThreads), smem, s, a) ==
-                 cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
+  // one CTA while each of its threads has a few rows at most (the cluster's
+  // barriers cost about 1 us), else a cluster of eight
+  if (a.n_rows + a.n_req <= 4 * kPlanThreads)
+    return launch_k(k_paged_plan, dim3(1), dim3(kPlanThreads), smem, s, a) ==
+                   cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
+  return launch_cluster(kPlanCluster, k_paged_plan, dim3(kPlanCluster), dim3(kPlanThreads),
+                        smem, s, a) == cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
 }
 
 // ---------------------------------------------------------------- append --
 
-SLX_DEV uint8_t f32_to_e4m3(float x) {
-  return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+SLX_DEV uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One CTA per row.  The row's hd / 2 rotations once in shared memory (angle
-// in fp64, reduced to one turn, then fp32 sine and cosine), then hd / 8
-// lanes per head, eight elements each: the other half of a rotated pair sits
-// hd / 16 lanes away.
-constexpr int kAppendThreads = 256;
+// four values to e4m3, to nearest, saturating at 448
+SLX_DEV uint32_t f32x4_to_e4m3(const float (&x)[4]) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+// One CTA per row, hd / 8 lanes per head, each with four elements of the
+// head's first half and the four they are rotated with.  The row's heads are
+// requested first; while they come, hd / 2 threads form the row's rotations
+// (the angle in turns, in fp64, less its whole turns).  Keys of e4m3 pages go
+// through fp64 up to their one rounding: with a step of 2^-3, a value that
+// fp32 leaves on the wrong side of a step's middle would be off by far more
+// than fp32's own error.  Bound by instruction issue for many rows, by the
+// chain position -> rotations -> barrier -> stores for few.
+constexpr int kAppendThreads = 128;
+constexpr int kAppendAhead = 4;  // passes over the heads requested together
+
+// Four elements of each half of a head (bf16).
+struct HalfPair {
+  uint2 a, b;
+  template <typename R>
+  SLX_DEV void get(R (&x)[4], R (&y)[4]) const {
+    x[0] = bf16_lo(a.x); x[1] = bf16_hi(a.x); x[2] = bf16_lo(a.y); x[3] = bf16_hi(a.y);
+    y[0] = bf16_lo(b.x); y[1] = bf16_hi(b.x); y[2] = bf16_lo(b.y); y[3] = bf16_hi(b.y);
+  }
+};
 
 template <int HD, bool E4M3>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArgs a) {
-  constexpr int L = HD / 8;  // lanes per head
-  __shared__ float s_cos[HD / 2], s_sin[HD / 2];
+__global__ void __launch_bounds__(kAppendThreads, 8) k_paged_append(const AppendArgs a) {
+  constexpr int L = HD / 8;                // lanes per head
+  constexpr int PH = kAppendThreads / L;   // heads per pass
+  __shared__ __align__(16) float2 s_rot[HD / 2];  // cosine, sine
+  __shared__ __align__(16) double2 s_rot_k[E4M3 ? HD / 2 : 1];  // the keys', where they are fp64
   pdl_launch_dependents();
+  const int l = threadIdx.x % L, lh = threadIdx.x / L;
+  auto load = [&](const uint16_t* head) {
+    return HalfPair{reinterpret_cast<const uint2*>(head)[l],
+                    reinterpret_cast<const uint2*>(head + HD / 2)[l]};
+  };
+  // fixed inputs, before the wait
+  const HalfPair wq = load(a.qn), wk = load(a.kn);
+  const double freq = threadIdx.x < HD / 2 ? (double)a.inv_freq[threadIdx.x] : 0.0;
   pdl_wait_primary();
   const int t = blockIdx.x, nkv = a.kv.n_kv;
+  const uint16_t* row = a.qkv + (size_t)t * a.stride;
   const int p = a.pos[t];
-  int slot = p < 0 ? -1 : a.slot[t];
+  int slot = a.slot[t];
+  // the first pass over the keys and the first few over queries and values
+  // (head n of those: query n, then value n - nq)
+  const int rest = a.nq + nkv;
+  HalfPair k_raw = {}, raw[kAppendAhead] = {};
+  if (lh < nkv) k_raw = load(row + (a.nq + lh) * HD);
+  auto request = [&](int n0) {
+#pragma unroll
+    for (int i = 0; i < kAppendAhead; ++i) {
+      const int n = n0 + i * PH + lh;
+      if (n < rest) raw[i] = load(row + (n < a.nq ? n : n + nkv) * HD);
+    }
+  };
+  request(0);
   if (slot >= a.kv.n_pages * a.kv.page_size) {
-    if (threadIdx.x == 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+    if (threadIdx.x == 0 && p >= 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
     slot = -1;
   }
-  if (slot < 0) {
+  if (slot < 0 || p < 0) {
     uint4* q = reinterpret_cast<uint4*>(a.q_out + (size_t)t * a.nq * HD);
     for (int i = threadIdx.x; i < a.nq * L; i += kAppendThreads)
       q[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   if (threadIdx.x < HD / 2) {
-    const double turn = 6.283185307179586476925286766559;
-    double ang = (double)p * (double)a.inv_freq[threadIdx.x];
-    ang -= rint(ang * (1.0 / turn)) * turn;
-    float sn, cs;
-    sincosf((float)ang, &sn, &cs);
-    s_cos[threadIdx.x] = cs;
-    s_sin[threadIdx.x] = sn;
+    double turns = (double)p * freq * 0.15915494309189533577;  // / (2 pi)
+    turns -= rint(turns);
+    float2 r;
+    sincospif((float)(2.0 * turns), &r.y, &r.x);
+    s_rot[threadIdx.x] = r;
+    if constexpr (E4M3) sincospi(2.0 * turns, &s_rot_k[threadIdx.x].y, &s_rot_k[threadIdx.x].x);
   }
   __syncthreads();
-  const int l = threadIdx.x % L;
-  const uint16_t* row = a.qkv + (size_t)t * a.stride;
-  const size_t ps = a.kv.page_size;
-  const int page = slot / (int)ps, off = slot % (int)ps;
-  const int heads = a.nq + 2 * nkv;
-  // whole warps loop together (the head sums use shuffles)
-  for (int h0 = 0; h0 < heads; h0 += kAppendThreads / L) {
-    const int h = h0 + threadIdx.x / L;
-    const bool on = h < heads;
-    const uint4 raw = on ? reinterpret_cast<const uint4*>(row + (size_t)h * HD)[l]
-                         : make_uint4(0, 0, 0, 0);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
+  float2 rot[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      x[2 * q] = bf16_lo(w[q]);
-      x[2 * q + 1] = bf16_hi(w[q]);
-    }
-    float ss = 0.f;
+  for (int j = 0; j < 4; ++j) rot[j] = s_rot[4 * l + j];
+  // a lane's share of a head in type R: RMSNorm (by(mean square) is the
+  // factor), then the rotation
+  auto rotated = [&](auto zero, const HalfPair& in, const HalfPair& weight, const auto* ro,
+                     float (&u)[4], float (&v)[4], auto by) {
+    using R = decltype(zero);
+    R x[4], y[4], wx[4], wy[4], ss = zero;
+    in.get(x, y);
+    weight.get(wx, wy);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+    for (int j = 0; j < 4; ++j) ss += x[j] * x[j] + y[j] * y[j];
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const bool is_v = h >= a.nq + nkv;
-    const uint16_t* nw = h < a.nq ? a.qn : a.kn;
-    const float inv = rsqrtf(ss / (float)HD + a.eps);
-    float y[8];
+    const R f = by(ss / (R)HD + (R)a.eps);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float n = is_v ? x[j] : x[j] * inv * bf16_to_f32(nw[l * 8 + j]);
-      const float other = __shfl_xor_sync(0xffffffffu, n, L / 2);
-      const int i = (l % (L / 2)) * 8 + j;
-      const float cs = s_cos[i], sn = s_sin[i];
-      // first half a cos - b sin, second half b cos + a sin
-      y[j] = is_v ? n : l < L / 2 ? n * cs - other * sn : n * cs + other * sn;
+    for (int j = 0; j < 4; ++j) {
+      const R n = x[j] * f * wx[j], m = y[j] * f * wy[j];
+      u[j] = (float)(n * ro[j].x - m * ro[j].y);
+      v[j] = (float)(n * ro[j].y + m * ro[j].x);
     }
-    if (!on) continue;
-    if (h < a.nq) {
-      uint4 o;
-      o.x = pack_bf16x2(y[0], y[1]);
-      o.y = pack_bf16x2(y[2], y[3]);
-      o.z = pack_bf16x2(y[4], y[5]);
-      o.w = pack_bf16x2(y[6], y[7]);
-      reinterpret_cast<uint4*>(a.q_out + ((size_t)t * a.nq + h) * HD)[l] = o;
-      continue;
-    }
-    const int kh = is_v ? h - a.nq - nkv : h - a.nq;
-    const size_t at = ((((size_t)page * 2 + is_v) * nkv + kh) * ps + off) * HD + l * 8;
-    if (E4M3) {
-      const float sc = is_v ? a.kv.v_scale[kh] : a.kv.k_scale[kh];
-      uint32_t o[2] = {0, 0};
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        o[j / 4] |= (uint32_t)f32_to_e4m3(y[j] / sc) << (8 * (j % 4));
-      *reinterpret_cast<uint2*>(a.kv.base + at) = make_uint2(o[0], o[1]);
+  };
+  auto half = [](const float (&x)[4]) {
+    return make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+  };
+  const int page = slot >> a.kv.page_shift, off = slot & (a.kv.page_size - 1);
+  auto put = [&](const float (&u)[4], const float (&v)[4], int kh, int is_v) {
+    const size_t at =
+        (((((size_t)page * 2 + is_v) * nkv + kh) << a.kv.page_shift) + off) * HD + 4 * l;
+    if constexpr (E4M3) {
+      *reinterpret_cast<uint32_t*>(a.kv.base + at) = f32x4_to_e4m3(u);
+      *reinterpret_cast<uint32_t*>(a.kv.base + at + HD / 2) = f32x4_to_e4m3(v);
     } else {
-      uint4 o;
-      o.x = pack_bf16x2(y[0], y[1]);
-      o.y = pack_bf16x2(y[2], y[3]);
-      o.z = pack_bf16x2(y[4], y[5]);
-      o.w = pack_bf16x2(y[6], y[7]);
-      *reinterpret_cast<uint4*>(a.kv.base + 2 * at) = o;
+      *reinterpret_cast<uint2*>(a.kv.base + 2 * at) = half(u);
+      *reinterpret_cast<uint2*>(a.kv.base + 2 * at + HD) = half(v);
+    }
+  };
+  float u[4], v[4];
+  for (int h0 = 0; h0 < nkv; h0 += PH) {
+    const int h = h0 + lh;
+    // (warps without a key have nothing to sum)
+    if (!__any_sync(0xffffffffu, h < nkv)) continue;
+    if (h0 > 0 && h < nkv) k_raw = load(row + (a.nq + h) * HD);
+    if constexpr (E4M3)
+      rotated(0.0, k_raw, wk, s_rot_k + 4 * l, u, v, [&](double ms) {
+        return rsqrt(ms) / (double)(h < nkv ? a.kv.k_scale[h] : 1.f);
+      });
+    else
+      rotated(0.f, k_raw, wk, rot, u, v, [](float ms) { return rsqrtf(ms); });
+    if (h < nkv) put(u, v, h, 0);
+  }
+  for (int n0 = 0; n0 < rest; n0 += kAppendAhead * PH) {
+    if (n0 > 0) request(n0);
+#pragma unroll
+    for (int i = 0; i < kAppendAhead; ++i) {
+      const int n = n0 + i * PH + lh;
+      if (__any_sync(0xffffffffu, n < a.nq)) {
+        rotated(0.f, raw[i], wq, rot, u, v, [](float ms) { return rsqrtf(ms); });
+        if (n < a.nq) {
+          uint2* q = reinterpret_cast<uint2*>(a.q_out + ((size_t)t * a.nq + n) * HD);
+          q[l] = half(u);
+          q[l + L] = half(v);
+        }
+      }
+      if (n >= a.nq && n < rest) {
+        raw[i].get(u, v);
+        if constexpr (E4M3) {
+          const float sc = a.kv.v_scale[n - a.nq];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            u[j] /= sc;
+            v[j] /= sc;
+          }
+        }
+        put(u, v, n - a.nq, 1);
+      }
     }
   }
 }
@@ -391,11 +474,6 @@ SLX_DEV void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{.reg .b16 t, u; mov.b32 {t, u}, %2; cvt.rn.f16x2.e4m3x2 %0, t; "
       "cvt.rn.f16x2.e4m3x2 %1, u;}"
       : "=r"(lo), "=r"(hi) : "r"(w));
-}
-
-SLX_DEV uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Row t's request and the keys it attends: pos + 1, 0 for an idle row or one
