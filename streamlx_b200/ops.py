@@ -225,6 +225,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _cur_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
+_status_words: dict = {}    # device index -> the word _status() keeps
+_ws_bytes: dict = {}        # (n_q, n_kv, head_dim) -> bytes, T > 0
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
@@ -246,12 +250,11 @@ def _call_status(status, idx: int) -> int:
     replay): its device errors are not reported."""
     if status is not None:
         return _vec(status, 1, _I32, idx, "status")
-    dev = torch.device("cuda", idx)
-    t = _scratch.get(("status", dev))
+    t = _status_words.get(idx)
     if t is None:
         if torch.cuda.is_current_stream_capturing():
             return 0
-        t = _status(dev)
+        t = _status_words[idx] = _status(torch.device("cuda", idx))
     return t.data_ptr()
 
 
@@ -307,8 +310,8 @@ def paged_plan(n_new: torch.Tensor, lengths: torch.Tensor,
     # rows (request, position, slot), their starts and the state after the
     # step, one allocation
     buf = torch.empty(3 * n_rows + 2 * R + 2, dtype=_I32, device=table.device)
-    req, pos, slot, start, ln, nf = buf.split(
-        (n_rows, n_rows, n_rows, R + 1, R, 1))
+    req, pos, slot, start, ln, nf = torch.split_with_sizes(
+        buf, (n_rows, n_rows, n_rows, R + 1, R, 1))
     if lengths_out is None:
         lengths_out = ln
     if n_free_out is None:
@@ -367,8 +370,8 @@ def paged_append(qkv: torch.Tensor, pages: torch.Tensor, slot: torch.Tensor,
 
 def paged_workspace(rows: int, n_q: int, n_kv: int, head_dim: int,
                     device) -> torch.Tensor:
-    """Workspace of paged_attention for up to ``rows`` rows, for callers
-    that must not allocate per call.  Its content does not matter; calls that
+    """Workspace of paged_attention for any number of rows up to ``rows``,
+    for callers that must not allocate per call.  Its content does not matter; calls that
     may overlap (streams, graphs) need one each."""
     n = L.paged_attn_workspace_bytes(rows, n_q, n_kv, head_dim)
     return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
@@ -413,9 +416,11 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor,
                          "n_q, head_dim]")
     if workspace is None:
         # the call's own: calls on other streams or in graphs share nothing
-        workspace = q.new_empty(
-            max(L.paged_attn_workspace_bytes(T, n_q, n_kv, hd), 16),
-            dtype=torch.uint8)
+        need = _ws_bytes.get((n_q, n_kv, hd))
+        if need is None:
+            need = max(L.paged_attn_workspace_bytes(1, n_q, n_kv, hd), 16)
+            _ws_bytes[n_q, n_kv, hd] = need
+        workspace = q.new_empty(need, dtype=torch.uint8)
     elif (workspace.dtype is not torch.uint8 or workspace.dim() != 1 or
           workspace.get_device() != idx or not workspace.is_contiguous()):
         raise ValueError("paged_attention: workspace must come from "
