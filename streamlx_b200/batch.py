@@ -1,0 +1,347 @@
+"""Several requests decoded together over a paged KV cache.
+
+``BatchDecoder`` drives a ``SynthDecoder`` (model.py) with rows of many
+requests per step: the plan of the step (``ops.paged_plan``: pages, block
+tables, slots), per layer the q/k norm + RoPE + append to the pages and the
+attention over them, the pool-backed experts on all rows (the reference's
+SwitchGLU wrapper takes any number of rows, streamlx/integrate.py:234-298), and
+the logits' penalties, biases and grammar masks with the greedy pick.  Prompts
+are fed in chunks beside the requests that already decode.  The reference
+decodes one request at a time (examples/generate.py:67-89).
+"""
+
+from __future__ import annotations
+
+from collections import deque
+from dataclasses import dataclass, field
+
+import numpy as np
+import torch
+
+from . import _lib as L
+from . import ops
+
+
+@dataclass
+class LogitRules:
+    """What one request's logits go through before the pick."""
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    bias: dict = field(default_factory=dict)    # id -> added logit
+    # grammar: called with the request's output ids, returns uint32 words
+    # (bit i of word w allows id 32 w + i) or None for "anything"
+    mask: object = None
+
+
+class PagedKVCache:
+    """KV pages of every layer and the state of their requests, on the GPU.
+    E4m3 pages hold value / scale; ``kv_scale`` [2, kv_heads] per layer."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, *,
+                 n_pages: int, page_size: int, max_requests: int,
+                 max_tokens: int, dtype=torch.bfloat16, kv_scale=None,
+                 device=None):
+        if page_size not in ops.PAGE_SIZES:
+            raise ValueError(f"page_size {page_size}: one of {ops.PAGE_SIZES}")
+        if dtype == torch.float8_e4m3fn and kv_scale is None:
+            raise ValueError("an e4m3 cache needs kv_scale")
+        self.page_size, self.n_pages = page_size, n_pages
+        self.pages = [torch.zeros(n_pages, 2, kv_heads, page_size, head_dim,
+                                  dtype=dtype, device=device)
+                      for _ in range(layers)]
+        self.kv_scale = kv_scale or [None] * layers
+        i32 = dict(dtype=torch.int32, device=device)
+        cols = self.pages_for(max_tokens)
+        self.table = torch.full((max_requests, cols), -1, **i32)
+        self.lengths = torch.zeros(max_requests, **i32)
+        # popped from the end: page 0 first
+        self.free_list = torch.arange(n_pages - 1, -1, -1, **i32)
+        self.n_free = torch.full((1,), n_pages, **i32)
+
+    def pages_for(self, tokens: int) -> int:
+        return (tokens + self.page_size - 1) // self.page_size
+
+    def plan(self, n_new: torch.Tensor, n_rows: int, status) -> ops.PagedPlan:
+        """Rows of a step; the cache's lengths and free pages move on."""
+        return ops.paged_plan(n_new, self.lengths, self.table, self.free_list,
+                              self.n_free, self.page_size, n_rows,
+                              lengths_out=self.lengths, n_free_out=self.n_free,
+                              status=status)
+
+
+class _Request:
+    def __init__(self, rid, prompt, max_new, rules, eos):
+        self.rid, self.prompt, self.max_new = rid, prompt, max_new
+        self.rules, self.eos = rules, eos
+        self.fed = 0                # tokens in the cache
+        self.out: list[int] = []
+
+
+class BatchDecoder:
+    """Decodes up to ``max_requests`` requests of a decoder together.
+
+    ``submit`` queues a request, ``step`` runs one step and returns the tokens
+    it picked, ``generate`` runs a list of prompts to their ends.  A request
+    is admitted when the pages of its prompt and ``max_new`` tokens are free,
+    so a running one never runs out.  The pools' bookkeeping is the eager
+    path's (one host sync on the routed ids per layer); single-request decode
+    through the step graph stays ``SynthDecoder.step``."""
+
+    def __init__(self, model, max_requests: int = 8, max_tokens: int = 1024,
+                 n_pages: int | None = None, page_size: int = 64,
+                 cache_dtype=torch.bfloat16, kv_scale=None,
+                 prompt_chunk: int = 64):
+        cfg = model.cfg
+        if not cfg.has_trunk:
+            raise ValueError("batched decode needs a decoder with attention")
+        if model.ep is not None:
+            raise ValueError("batched decode runs on one GPU: the experts of "
+                             "this model are sharded")
+        if max_requests < 1 or max_tokens < 1 or prompt_chunk < 1:
+            raise ValueError("max_requests, max_tokens and prompt_chunk must "
+                             "be positive")
+        self.model, self.cfg, self.device = model, cfg, model.device
+        self.max_tokens, self.chunk = max_tokens, prompt_chunk
+        if n_pages is None:
+            n_pages = max_requests * ((max_tokens + page_size - 1) // page_size)
+        if cache_dtype == torch.float8_e4m3fn and kv_scale is None:
+            kv_scale = [self._key_scale(la) for la in model.layers]
+        self.cache = PagedKVCache(
+            cfg.layers, cfg.kv_heads, cfg.head_dim, n_pages=n_pages,
+            page_size=page_size, max_requests=max_requests,
+            max_tokens=max_tokens, dtype=cache_dtype, kv_scale=kv_scale,
+            device=self.device)
+        self.slots: list[_Request | None] = [None] * max_requests
+        self._gone: set[int] = set()    # slots whose pages go back next step
+        self._queue: deque = deque()
+        self._next_id = 0
+        self._reserved = 0              # pages promised to running requests
+        i32 = dict(dtype=torch.int32, device=self.device)
+        self.status = torch.zeros(1, **i32)
+        self.history = torch.zeros(max_requests, max_tokens, **i32)
+        self.last = torch.zeros(max_requests, **i32)    # last picked tokens
+        self.logits: torch.Tensor | None = None     # of the last step's picks
+        self.logits_of: list[int] = []              # their request ids
+
+    def _key_scale(self, layer) -> torch.Tensor:
+        """A key leaves the RMSNorm with at most sqrt(head_dim) times the
+        largest norm weight, so this scale keeps it within e4m3's 448;
+        values keep scale 1."""
+        kv, hd = self.cfg.kv_heads, self.cfg.head_dim
+        s = torch.ones(2, kv, device=self.device)
+        s[0] = layer.k_norm.float().abs().max() * hd ** 0.5 / 448
+        return s
+
+    # ------------------------------------------------------------ requests --
+
+    def submit(self, prompt, max_new: int, rules: LogitRules | None = None,
+               eos: int | None = None) -> int:
+        """Queue a request; returns its id."""
+        prompt = [int(t) for t in prompt]
+        if not prompt or max_new < 1:
+            raise ValueError("a request needs a prompt and max_new >= 1")
+        if any(not 0 <= t < self.cfg.vocab for t in prompt):
+            raise ValueError("prompt token outside the vocabulary")
+        total = len(prompt) + max_new
+        if total > self.max_tokens or \
+                self.cache.pages_for(total) > self.cache.n_pages:
+            raise ValueError(f"{total} tokens do not fit the cache "
+                             f"({self.max_tokens} a request, "
+                             f"{self.cache.n_pages} pages)")
+        r = _Request(self._next_id, prompt, max_new, rules, eos)
+        self._next_id += 1
+        self._queue.append(r)
+        return r.rid
+
+    def _pages(self, r: _Request) -> int:
+        return self.cache.pages_for(len(r.prompt) + r.max_new)
+
+    def _admit(self) -> None:
+        for s, r in enumerate(self.slots):
+            if not self._queue:
+                return
+            if r is not None or s in self._gone:
+                continue
+            new = self._queue[0]
+            if self._reserved + self._pages(new) > self.cache.n_pages:
+                return
+            self._queue.popleft()
+            self._reserved += self._pages(new)
+            self.slots[s] = new
+            self.history[s, :len(new.prompt)] = torch.tensor(
+                new.prompt, dtype=torch.int32, device=self.device)
+
+    @property
+    def busy(self) -> bool:
+        return bool(self._queue) or any(r is not None for r in self.slots)
+
+    # ---------------------------------------------------------------- step --
+
+    @torch.no_grad()
+    def step(self) -> dict[int, int]:
+        """One step of every running request: its next prompt chunk, or its
+        last token.  Returns {request id: picked token} of the requests past
+        their prompts; a request whose mask allows nothing ends with -1."""
+        with torch.cuda.device(self.device):
+            return self._step()
+
+    def _step(self) -> dict[int, int]:
+        self.model.flush()
+        self._admit()
+        n_new, ids, from_last, picking = [], [], [], []
+        for s, r in enumerate(self.slots):
+            if r is None:
+                n_new.append(-1 if s in self._gone else 0)
+                continue
+            left = len(r.prompt) - r.fed
+            n = min(left, self.chunk) if left > 0 else 1
+            n_new.append(n)
+            if left > 0:
+                ids += r.prompt[r.fed:r.fed + n]
+            else:
+                from_last.append((len(ids), s))
+                ids.append(0)
+            r.fed += n
+            if left <= n:
+                picking.append((s, len(ids) - 1))   # slot, its last row
+        dev = self.device
+        rows = len(ids)
+        plan = self.cache.plan(torch.tensor(n_new, dtype=torch.int32).to(dev),
+                               rows, self.status)
+        self._gone.clear()
+        if rows == 0:
+            self._check()
+            return {}
+        tok = torch.tensor(ids, dtype=torch.int32).to(dev)
+        if from_last:
+            at, slot = (torch.tensor(v, device=dev) for v in zip(*from_last))
+            tok[at] = self.last[slot]
+        x = self._forward(tok, plan)
+        if not picking:
+            self._check()
+            return {}
+        slots, last = zip(*picking)
+        self.logits_of = [self.slots[s].rid for s in slots]
+        x = x[torch.tensor(last, device=dev)].contiguous()
+        self.logits = torch.empty(len(slots), self.cfg.vocab,
+                                  dtype=torch.bfloat16, device=dev)
+        L.qlinear(self.model.w_lm, self.cfg.vocab, self.cfg.hidden,
+                  self.cfg.trunk_bits, x, self.logits, self.status)
+        return self._pick(slots)
+
+    def _forward(self, tok, plan) -> torch.Tensor:
+        """Hidden rows (after the final norm) of the step's tokens."""
+        m, cfg, dev, st = self.model, self.cfg, self.device, self.status
+        T, H, hd, bits = tok.shape[0], cfg.hidden, cfg.head_dim, cfg.trunk_bits
+        bf = dict(dtype=torch.bfloat16, device=dev)
+        h, x = torch.empty(T, H, **bf), torch.empty(T, H, **bf)
+        L.dequant_rows(m.embed, H, bits, tok, T, cfg.vocab, h, st)
+        qkv = torch.empty(T, (cfg.heads + 2 * cfg.kv_heads) * hd, **bf)
+        att = torch.empty(T, cfg.heads, hd, **bf)
+        o = torch.empty(T, H, **bf)
+        work = ops.paged_workspace(T, cfg.heads, cfg.kv_heads, hd, dev)
+        ids = torch.empty(T, cfg.top_k, dtype=torch.int32, device=dev)
+        scores = torch.empty(T, cfg.top_k, dtype=torch.float32, device=dev)
+        scratch = torch.zeros(L.router_scratch_bytes(T, cfg.n_experts),
+                              dtype=torch.uint8, device=dev)
+        delta = None
+        for i, la in enumerate(m.layers):
+            pages, scale = self.cache.pages[i], self.cache.kv_scale[i]
+            L.add_rmsnorm(h, delta, la.w_in, cfg.rms_eps, x)
+            L.qlinear(la.w_qkv, la.n_qkv, H, bits, x, qkv, st)
+            q = ops.paged_append(qkv, pages, plan.slot, plan.pos, cfg.heads,
+                                 la.q_norm, la.k_norm, cfg.rms_eps,
+                                 m.inv_freq, kv_scale=scale, status=st)
+            ops.paged_attention(q, pages, self.cache.table, plan.pos,
+                                req=plan.req, kv_scale=scale, out=att,
+                                workspace=work, status=st)
+            L.qlinear(la.w_o, H, cfg.heads * hd, bits, att, o, st, T=T)
+            L.add_rmsnorm(h, o, la.post_attention_layernorm, cfg.rms_eps, x)
+            blk = la.mlp
+            L.router_topk(x, blk.w_gate, blk.bias, cfg.top_k,
+                          cfg.norm_topk_prob, ids, scores, scratch, st)
+            delta = blk.switch_mlp.fused(x[None], scores[None], ids[None])[0]
+        L.add_rmsnorm(h, delta, m.norm, cfg.rms_eps, x)
+        return x
+
+    def _pick(self, slots) -> dict[int, int]:
+        """Rules, greedy pick and the requests' state after it."""
+        dev, V = self.device, self.cfg.vocab
+        reqs = [self.slots[s] for s in slots]
+        rules = [r.rules or LogitRules() for r in reqs]
+        at = torch.tensor(slots, device=dev)
+        n_hist = [len(r.prompt) + len(r.out) for r in reqs]
+        kw = {}
+        if any(u.repetition != 1 or u.frequency or u.presence for u in rules):
+            kw = {name: torch.tensor([getattr(u, name) for u in rules],
+                                     dtype=torch.float32).to(dev)
+                  for name in ("repetition", "frequency", "presence")}
+            kw["history"] = self.history[at, :max(n_hist)].contiguous()
+            kw["n_prompt"] = torch.tensor([len(r.prompt) for r in reqs],
+                                          dtype=torch.int32).to(dev)
+            kw["n_history"] = torch.tensor(n_hist, dtype=torch.int32).to(dev)
+        if any(u.bias for u in rules):
+            b = [list(u.bias.items()) for u in rules]
+            start = np.cumsum([0] + [len(e) for e in b]).astype(np.int32)
+            ids, vals = zip(*[e for row in b for e in row])
+            kw["bias"] = (torch.tensor(ids, dtype=torch.int32).to(dev),
+                          torch.tensor(vals, dtype=torch.float32).to(dev),
+                          torch.from_numpy(start).to(dev))
+        if any(u.mask is not None for u in rules):
+            words = (V + 31) // 32
+            m = np.full((len(reqs), words), 0xFFFFFFFF, dtype=np.uint32)
+            for i, (r, u) in enumerate(zip(reqs, rules)):
+                w = u.mask(list(r.out)) if u.mask is not None else None
+                if w is not None:
+                    m[i] = np.asarray(w, dtype=np.uint32)[:words]
+            kw["mask"] = torch.from_numpy(m.view(np.int32)).to(dev)
+        pick = ops.process_logits(self.logits, status=self.status, **kw)
+        self.last[at] = pick
+        # the picked token's place: its request's history goes on with it
+        hist = torch.tensor(n_hist, device=dev).clamp(max=self.max_tokens - 1)
+        self.history[at, hist] = pick
+        got = pick.tolist()
+        self._check()
+        for s, r, t in zip(slots, reqs, got):
+            r.out.append(t)
+            if t < 0 or t == r.eos or len(r.out) >= r.max_new:
+                self._reserved -= self._pages(r)
+                self.slots[s] = None
+                self._gone.add(s)
+        return {r.rid: t for r, t in zip(reqs, got)}
+
+    def _check(self) -> None:
+        ops.check_status(self.device)
+        code = int(self.status.item())
+        if code != 0:
+            self.status.zero_()
+            raise L.SlxError("device", code, "batched decode step device error")
+
+    # ------------------------------------------------------------ generate --
+
+    def generate(self, prompts, max_new: int, rules=None,
+                 eos: int | None = None) -> list[list[int]]:
+        """Every prompt to its end; ``rules``: one LogitRules, or one per
+        prompt.  A mask that allows nothing ends a request without a token."""
+        if not isinstance(rules, (list, tuple)):
+            rules = [rules] * len(prompts)
+        if len(rules) != len(prompts):
+            raise ValueError("one LogitRules per prompt")
+        ids = [self.submit(p, max_new, r, eos) for p, r in zip(prompts, rules)]
+        out: dict = {i: [] for i in ids}
+        while self.busy:
+            for rid, t in self.step().items():
+                if t >= 0 and rid in out:
+                    out[rid].append(t)
+        self.release()
+        return [out[i] for i in ids]
+
+    def release(self) -> None:
+        """Hand the finished requests' pages back now (a step does, too)."""
+        if self._gone:
+            n = [-1 if s in self._gone else 0 for s in range(len(self.slots))]
+            with torch.cuda.device(self.device):
+                self.cache.plan(torch.tensor(n, dtype=torch.int32).to(
+                    self.device), 0, self.status)
+            self._gone.clear()

@@ -815,6 +815,19 @@ class SynthDecoder:
         self.flush()
         return out
 
+    def generate_batch(self, prompts, max_new: int, rules=None,
+                       eos: int | None = None, **cache) -> list[list[int]]:
+        """Greedy decode of several prompts together over a paged KV cache
+        (batch.BatchDecoder; ``cache``: its page_size, cache_dtype, ...).
+        ``rules``: a batch.LogitRules for all prompts, or one per prompt."""
+        from .batch import BatchDecoder
+        prompts = [list(p) for p in prompts]
+        longest = max((len(p) for p in prompts), default=0) + max_new
+        cache.setdefault("max_tokens", max(longest, 1))
+        cache.setdefault("max_requests", max(min(len(prompts), 64), 1))
+        return BatchDecoder(self, **cache).generate(prompts, max_new, rules,
+                                                    eos)
+
     @torch.no_grad()
     def moe_forward(self, layer: int, x: torch.Tensor) -> torch.Tensor:
         """MoE block of one layer on hidden rows x [T, H] (router, experts,
