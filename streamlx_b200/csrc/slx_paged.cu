@@ -405,11 +405,18 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // same request (a prompt's rows share their keys: see group_of).
 //
 // The contraction index of an MMA may be permuted on both sides alike; the
-// fragments are chosen so that each is 16 contiguous bytes of a key: keys and
-// values go from global memory to fragments without shared memory, the next
-// unit's into the registers that this one's have just left.  V pairs two keys
-// per register (byte permutes); S^T's accumulators become P^T's operand by
-// movmatrix.
+// fragments are chosen so that each is 16 contiguous bytes of a key.
+//   bf16: keys and values go from global memory to fragments without shared
+//   memory, the next unit's into the registers that this one's have just left
+//   (482 us for 256 requests of 6k tokens, 24/4 heads; through the ring below
+//   499).
+//   e4m3: half the bytes and twice the work per byte.  A unit's keys and its
+//   values are one contiguous block each: every warp has a ring of stages in
+//   shared memory that its first lane fills by bulk copies, some units ahead
+//   and across the ends of rows (111 us for 128 requests of 1k to 16k tokens,
+//   16/2 heads; with register loads 134).
+// V pairs two keys per register (byte permutes); S^T's accumulators become
+// P^T's operand by movmatrix.
 //
 // P is rounded to two 16-bit parts (hi + lo: 16 bits or more in all), so the
 // only rounding of note is the output's.  E4m3 keys and values become fp16
@@ -424,7 +431,9 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = 32 * kPaWarps;
-constexpr int kPaUnit = 16;   // keys: what one MMA takes
+constexpr int kPaStages = 2;  // of a warp's ring
+// 16-key halves of a unit: as many bytes in flight either way
+constexpr int pa_halves(bool e4m3) { return e4m3 ? 2 : 1; }
 
 struct PaWork {       // workspace of one call
   int4* desc;         // [n] split (group, kv head): first, last CTA, row, head
@@ -438,14 +447,9 @@ SLX_DEV float exp2_fast(float x) {
   return y;
 }
 
-template <int B>
 SLX_DEV void ld_stream(const uint8_t* p, uint32_t* v) {
-  if constexpr (B == 16)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-                 : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
 }
 
 template <bool BF16>
@@ -475,6 +479,7 @@ SLX_DEV void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
       "cvt.rn.f16x2.e4m3x2 %1, u;}"
       : "=r"(lo), "=r"(hi) : "r"(w));
 }
+
 
 // Row t's request and the keys it attends: pos + 1, 0 for an idle row or one
 // out of range.  (Both are read at once: rows are read in batches.)
@@ -522,7 +527,7 @@ SLX_DEV long long warp_sum(int n) {
 
 // A run of units of one (row group, kv head) that falls to this CTA.
 struct PaSeg {
-  int row, kh, u0, u1, units, keys;
+  int row, kh, u0, u1, units, keys, req;
 };
 
 template <int HD, bool E4M3, int NT>
@@ -536,8 +541,15 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   constexpr int VB = RB >= 128 ? 16 : 8; // bytes of a piece of V
   constexpr int VP = RB / (8 * VB);      // its pieces per key
   constexpr int VW = RB / 32;            // words per lane and key
+  constexpr bool RING = E4M3;
+  constexpr int H = pa_halves(E4M3), kPaUnit = 16 * H;
+  constexpr int SB = 2 * kPaUnit * RB;   // a unit's keys, then its values
+  constexpr int S = RING ? kPaStages : 1;
+  extern __shared__ __align__(128) uint8_t pa_smem[];
   // merging the warps' states: two of them at a time, as they lie in registers
-  __shared__ float4 s_acc[kPaWarps / 2][NT * MT * 32];
+  float4* s_acc = reinterpret_cast<float4*>(pa_smem + (RING ? kPaWarps * S * SB : 0));
+  __shared__ __align__(8) uint64_t s_bar[kPaWarps][S];
+  __shared__ int s_bad[kPaWarps][S];     // halves of the stage without a page
   __shared__ float s_ml[2][2][8 * NT];
   __shared__ long long s_pre[kPaThreads + 1];
   __shared__ long long w_sum[kPaWarps];
@@ -602,7 +614,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   int4 my_desc = make_int4(-1, 0, 0, 0);
   if (x < x_end) {
     PaSeg sg;
-    int rb = 0, req;
+    int rb = 0;
     {
       // the group unit x is in: its run of tiles, then tile by tile
       long long before = 0;
@@ -635,7 +647,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
         before += __shfl_sync(0xffffffffu, v, 31) * nkv;
       }
       sg.keys = __shfl_sync(0xffffffffu, len_l, sg.row - rb);
-      req = __shfl_sync(0xffffffffu, rk.req, sg.row - rb);
+      sg.req = __shfl_sync(0xffffffffu, rk.req, sg.row - rb);
       sg.units = units_of(sg.keys);
       const long long in = x - before;
       sg.kh = in < 0x7fffffff ? (int)((unsigned)in / (unsigned)sg.units)
@@ -644,72 +656,170 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
       sg.u1 = (int)min((long long)sg.units, sg.u0 + (x_end - x));
     }
     const size_t page_bytes = (size_t)2 * nkv * ps * RB, v_off = (size_t)nkv * ps * RB;
-    // this lane's pieces of keys g, g + 8 and of values 2c, 2c + 1, 2c + 8, 2c + 9
-    uint32_t kr[2][KQ][4], vr[4][VW];
-    const int k_at = g * RB + c * 16, v_at = 2 * c * RB + g * VB;
-    const int32_t* tab = nullptr;
-    const uint8_t* head = nullptr;        // the kv head's keys in page 0
-    auto segment = [&] {
-      tab = a.table + (size_t)req * a.max_pages;
-      head = a.kv.base + (size_t)sg.kh * ps * RB;
+    // a place in the CTA's segments: the rows of tile rb and x as above
+    struct Place {
+      PaSeg sg;
+      int rb, len, req;  // len, req: of row rb + lane
+      long long x;
     };
-    // page of unit u of the segment (-1 behind its end)
-    auto page_of = [&](int u) { return u < sg.u1 ? tab[(u * kPaUnit) >> sh] : -1; };
+    // to the next segment; false behind the last
+    auto advance = [&](Place& p) {
+      p.x += p.sg.u1 - p.sg.u0;
+      if (p.x >= x_end) return false;
+      p.sg.u0 = 0;
+      if (++p.sg.kh == nkv) {
+        p.sg.kh = 0;
+        unsigned hit = __ballot_sync(0xffffffffu, p.len > 0 && p.rb + lane > p.sg.row);
+        while (!hit) {  // there is one: x < total
+          p.rb += 32;
+          const RowKeys r = row_keys(a, p.rb + lane);
+          p.len = lead_keys(r.keys, r.req, rpb);
+          p.req = r.req;
+          hit = __ballot_sync(0xffffffffu, p.len > 0);
+        }
+        const int i = __ffs(hit) - 1;
+        p.sg.row = p.rb + i;
+        p.sg.keys = __shfl_sync(0xffffffffu, p.len, i);
+        p.sg.req = __shfl_sync(0xffffffffu, p.req, i);
+        p.sg.units = units_of(p.sg.keys);
+      }
+      p.sg.u1 = (int)min((long long)p.sg.units, x_end - p.x);
+      return true;
+    };
+    Place at = {sg, rb, len_l, rk.req, x};   // what is computed
+    uint32_t vr[4][VW];  // words of values 2c, 2c + 1, 2c + 8, 2c + 9
+    // ---- register loads (bf16; units of 16 keys)
+    uint32_t kr[RING ? 1 : 2][KQ][4];        // pieces of keys g, g + 8
+    // page of unit u of the current segment
+    auto page_of = [&](int u) {
+      return u < at.sg.u1 ? a.table[(size_t)at.sg.req * a.max_pages + ((u * kPaUnit) >> sh)] : -1;
+    };
     auto keys_at = [&](int u, int page) {
-      return head + (size_t)(unsigned)page * page_bytes + ((u * kPaUnit) & (ps - 1)) * RB;
+      return a.kv.base + (size_t)(unsigned)page * page_bytes +
+             ((size_t)at.sg.kh * ps + ((u * kPaUnit) & (ps - 1))) * RB;
     };
-    // A unit's last key held by the group, -1 for a page out of range (zeros).
+    // the unit's last key that the group holds, -1 for a page out of range
     auto last_of = [&](int u, int page) {
-      if ((unsigned)page < (unsigned)a.kv.n_pages) return min(kPaUnit, sg.keys - u * kPaUnit) - 1;
+      if ((unsigned)page < (unsigned)a.kv.n_pages)
+        return min(kPaUnit, at.sg.keys - u * kPaUnit) - 1;
       if (lane == 0) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
       return -1;
     };
     auto load_k = [&](int u, int page) {
-      const int last = last_of(u, page);
-      if (last == kPaUnit - 1) {
-        const uint8_t* p = keys_at(u, page) + k_at;
+      if constexpr (!RING) {
+        const int last = last_of(u, page);
+        const uint8_t* p = keys_at(u, last < 0 ? 0 : page) + g * RB + c * 16;
+        if (last == kPaUnit - 1) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int q = 0; q < KQ; ++q) ld_stream<16>(p + r * 8 * RB + q * 64, kr[r][q]);
-      } else {
-        const uint8_t* p = keys_at(u, last < 0 ? 0 : page) + c * 16;
+            for (int q = 0; q < KQ; ++q) ld_stream(p + r * 8 * RB + q * 64, kr[r][q]);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int q = 0; q < KQ; ++q) {
-            kr[r][q][0] = kr[r][q][1] = kr[r][q][2] = kr[r][q][3] = 0;
-            if (g + 8 * r <= last) ld_stream<16>(p + (g + 8 * r) * RB + q * 64, kr[r][q]);
-          }
-      }
-    };
-    auto load_v = [&](int u, int page) {
-      const int last = last_of(u, page);
-      if (last == kPaUnit - 1) {
-        const uint8_t* p = keys_at(u, page) + v_off + v_at;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int q = 0; q < VP; ++q)
-            ld_stream<VB>(p + ((r & 1) + 8 * (r >> 1)) * RB + q * 128, vr[r] + q * (VB / 4));
-      } else {
-        const uint8_t* p = keys_at(u, last < 0 ? 0 : page) + v_off + g * VB;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = 2 * c + (r & 1) + 8 * (r >> 1);
-#pragma unroll
-          for (int q = 0; q < VW; ++q) vr[r][q] = 0;
-          if (key <= last) {
-#pragma unroll
-            for (int q = 0; q < VP; ++q) ld_stream<VB>(p + key * RB + q * 128, vr[r] + q * (VB / 4));
-          }
+            for (int q = 0; q < KQ; ++q) {
+              kr[r][q][0] = kr[r][q][1] = kr[r][q][2] = kr[r][q][3] = 0;
+              if (g + 8 * r <= last) ld_stream(p + r * 8 * RB + q * 64, kr[r][q]);
+            }
         }
       }
     };
-    segment();
-    int page = page_of(sg.u0 + warp);
-    bool loaded = false;                  // the first unit is on its way
+    auto load_v = [&](int u, int page) {
+      if constexpr (!RING) {
+        const int last = last_of(u, page);
+        const uint8_t* p = keys_at(u, last < 0 ? 0 : page) + v_off + 2 * c * RB + g * VB;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = (r & 1) + 8 * (r >> 1);
+          if (last < kPaUnit - 1) {
+#pragma unroll
+            for (int q = 0; q < VW; ++q) vr[r][q] = 0;
+            if (2 * c + key > last) continue;
+          }
+#pragma unroll
+          for (int q = 0; q < VP; ++q) ld_stream(p + key * RB + q * 128, vr[r] + q * 4);
+        }
+      }
+    };
+    int page = RING ? -1 : page_of(sg.u0 + warp);
+    bool loaded = false;                     // the segment's first unit is on its way
+    // ---- ring of bulk copies (e4m3)
+    Place ahead = at;                        // what is requested
+    uint8_t* ring = pa_smem + warp * (S * SB);
+    if (RING && lane == 0) {
+#pragma unroll
+      for (int i = 0; i < S; ++i) mbar_init(&s_bar[warp][i], 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+    int next_u = sg.u0 + warp, next_page[H];
+    bool live = true;
+    // this warp's next unit to request, and its page
+    auto seek = [&] {
+      while (next_u >= ahead.sg.u1) {
+        if (!advance(ahead)) {
+          live = false;
+          return;
+        }
+        next_u = warp;
+      }
+      const int32_t* tab = a.table + (size_t)ahead.sg.req * a.max_pages;
+      const int k0 = next_u * kPaUnit;
+      next_page[0] = tab[k0 >> sh];
+      // (a page of 16 keys is half a unit of 32)
+      if constexpr (H == 2)
+        next_page[1] = ps > 16 ? next_page[0] : k0 + 16 < ahead.sg.keys ? tab[(k0 + 16) >> sh] : 0;
+    };
+    auto request = [&](int st) {
+      if (!live) return;
+      if (lane == 0) {
+        const PaSeg& s = ahead.sg;
+        const int k0 = next_u * kPaUnit, held = min(kPaUnit, s.keys - k0);
+        uint64_t* bar = &s_bar[warp][st];
+        uint8_t* dst = ring + st * SB;
+        auto block = [&](int page, int k) {
+          return a.kv.base + (size_t)page * page_bytes +
+                 ((size_t)s.kh * ps + (k & (ps - 1))) * RB;
+        };
+        const bool one = H == 1 || ps > 16;     // the unit lies on one page
+        int bad = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+          if ((unsigned)next_page[h] >= (unsigned)a.kv.n_pages) bad |= 1 << h;
+        s_bad[warp][st] = bad;
+        if (bad) set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+        if (one && !bad) {
+          mbar_arrive_expect_tx(bar, 2 * held * RB);
+          const uint8_t* src = block(next_page[0], k0);
+          bulk_g2s_plain(dst, src, held * RB, bar);
+          bulk_g2s_plain(dst + kPaUnit * RB, src + v_off, held * RB, bar);
+        } else {
+          const int n0 = bad & 1 ? 0 : min(held, 16), n1 = one || (bad & 2) ? 0 : max(held - 16, 0);
+          mbar_arrive_expect_tx(bar, 2 * (n0 + n1) * RB);
+          if (n0) {
+            const uint8_t* src = block(next_page[0], k0);
+            bulk_g2s_plain(dst, src, n0 * RB, bar);
+            bulk_g2s_plain(dst + kPaUnit * RB, src + v_off, n0 * RB, bar);
+          }
+          if (n1) {
+            const uint8_t* src = block(next_page[H - 1], k0 + 16);
+            bulk_g2s_plain(dst + 16 * RB, src, n1 * RB, bar);
+            bulk_g2s_plain(dst + (kPaUnit + 16) * RB, src + v_off, n1 * RB, bar);
+          }
+        }
+      }
+      next_u += kPaWarps;
+      seek();
+    };
+    int used = 0;                            // units this warp has taken from it
+    if constexpr (RING) {
+      seek();
+#pragma unroll
+      for (int i = 0; i < S; ++i) request(i);
+    }
     while (true) {
+      sg = at.sg;
       int u = sg.u0 + warp;
       // columns n of the MMAs: row n / G of the group, q head n % G
       uint32_t qf[NT][KS][2];
@@ -724,7 +834,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
         if (rpb > 1) {
           row += n / G;
           const RowKeys r = row_keys(a, row);
-          keys = n < cols && row / rpb == sg.row / rpb && r.req == req ? r.keys : 0;
+          keys = n < cols && row / rpb == sg.row / rpb && r.req == sg.req ? r.keys : 0;
         }
         lim[nt][0] = __shfl_sync(0xffffffffu, keys, 8 * c);
         lim[nt][1] = __shfl_sync(0xffffffffu, keys, 8 * c + 4);
@@ -739,11 +849,13 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
                                                 : q * 64 + c * 16))
                                : make_uint4(0, 0, 0, 0);
       }
-      if (u < sg.u1 && !loaded) {
-        load_k(u, page);
-        load_v(u, page);
+      if constexpr (!RING) {
+        if (u < sg.u1 && !loaded) {
+          load_k(u, page);
+          load_v(u, page);
+        }
+        page = page_of(u + kPaWarps);
       }
-      page = page_of(u + kPaWarps);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if constexpr (!E4M3) {
@@ -804,56 +916,89 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
       }
       for (; u < sg.u1; u += kPaWarps) {
-        const int k0 = u * kPaUnit;
-        float s[NT][4], s2[NT][4];  // even and odd steps: two shorter chains
+        const int k0 = u * kPaUnit, st = used % S;
+        int bad = 0;                         // halves of the unit without a page
+        if constexpr (RING) {
+          mbar_wait(&s_bar[warp][st], used / S & 1, a.status);
+          bad = s_bad[warp][st];
+          ++used;
+        }
+        const uint8_t* sk = ring + st * SB + g * RB + c * 16;
+        const uint8_t* sv = ring + st * SB + kPaUnit * RB + 2 * c * RB + g * VB;
+        float s[NT][H][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < H; ++h) {
+          float s2[NT][4];  // even and odd steps: two shorter chains
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int q = 0; q < KQ; ++q) {
-          const uint32_t(&lo)[4] = kr[0][q];
-          const uint32_t(&hi)[4] = kr[1][q];
-          if constexpr (!E4M3) {
+            for (int i = 0; i < 4; ++i) s[nt][h][i] = s2[nt][i] = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<true>(s[nt], lo[0], hi[0], lo[1], hi[1], qf[nt][2 * q][0], qf[nt][2 * q][1]);
-              mma16816<true>(s2[nt], lo[2], hi[2], lo[3], hi[3], qf[nt][2 * q + 1][0],
-                             qf[nt][2 * q + 1][1]);
+          for (int q = 0; q < KQ; ++q) {
+            uint32_t lo[4], hi[4];  // pieces of keys g, g + 8
+            if constexpr (RING) {
+              const uint4 x0 = *reinterpret_cast<const uint4*>(sk + 16 * h * RB + q * 64);
+              const uint4 x1 = *reinterpret_cast<const uint4*>(sk + (16 * h + 8) * RB + q * 64);
+              lo[0] = x0.x; lo[1] = x0.y; lo[2] = x0.z; lo[3] = x0.w;
+              hi[0] = x1.x; hi[1] = x1.y; hi[2] = x1.z; hi[3] = x1.w;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                lo[i] = kr[0][q][i];
+                hi[i] = kr[RING ? 0 : 1][q][i];
+              }
             }
-          } else {
+            if constexpr (!E4M3) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a0, a1, a2, a3;
-              e4m3x4(lo[i], a0, a2);
-              e4m3x4(hi[i], a1, a3);
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<true>(s[nt][h], lo[0], hi[0], lo[1], hi[1], qf[nt][2 * q][0],
+                               qf[nt][2 * q][1]);
+                mma16816<true>(s2[nt], lo[2], hi[2], lo[3], hi[3], qf[nt][2 * q + 1][0],
+                               qf[nt][2 * q + 1][1]);
+              }
+            } else {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816<false>(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][4 * q + i][0],
-                                qf[nt][4 * q + i][1]);
+              for (int i = 0; i < 4; ++i) {
+                uint32_t a0, a1, a2, a3;
+                e4m3x4(lo[i], a0, a2);
+                e4m3x4(hi[i], a1, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816<false>(i & 1 ? s2[nt] : s[nt][h], a0, a1, a2, a3,
+                                  qf[nt][4 * q + i][0], qf[nt][4 * q + i][1]);
+              }
             }
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[nt][h][i] = (s[nt][h][i] + s2[nt][i]) * fac[nt][i & 1];
+              // a page out of range holds zeros
+              if (bad >> h & 1) s[nt][h][i] = 0.f;
+            }
         }
-        const int pg = page;
         const bool more_u = u + kPaWarps < sg.u1;
-        if (more_u) {
+        const int pg = page;
+        if (!RING && more_u) {
           load_k(u + kPaWarps, pg);
           page = page_of(u + 2 * kPaWarps);
         }
-        uint32_t ph[NT][2], pl[NT][2];  // P^T operands: hi and lo parts
+        uint32_t ph[NT][H][2], pl[NT][H][2];  // P^T operands: hi and lo parts
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * fac[nt][i & 1];
           if (k0 + kPaUnit > common) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (k0 + 8 * (i >> 1) + g >= lim[nt][i & 1]) s[nt][i] = -INFINITY;
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (k0 + 16 * h + 8 * (i >> 1) + g >= lim[nt][i & 1]) s[nt][h][i] = -INFINITY;
           }
           float f[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float mx = fmaxf(s[nt][i], s[nt][i + 2]);
+            float mx = fmaxf(s[nt][0][i], s[nt][0][i + 2]);
+            if constexpr (H == 2) mx = fmaxf(mx, fmaxf(s[nt][H - 1][i], s[nt][H - 1][i + 2]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -861,9 +1006,14 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
             const float ms = mx == -INFINITY ? 0.f : mx;
             f[i] = exp2_fast(m[nt][i] - ms);
             m[nt][i] = mx;
-            s[nt][i] = exp2_fast(s[nt][i] - ms);
-            s[nt][i + 2] = exp2_fast(s[nt][i + 2] - ms);
-            l[nt][i] = l[nt][i] * f[i] + (s[nt][i] + s[nt][i + 2]);
+            float sum = 0.f;
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+              s[nt][h][i] = exp2_fast(s[nt][h][i] - ms);
+              s[nt][h][i + 2] = exp2_fast(s[nt][h][i + 2] - ms);
+              sum += s[nt][h][i] + s[nt][h][i + 2];
+            }
+            l[nt][i] = l[nt][i] * f[i] + sum;
           }
           if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
@@ -875,20 +1025,22 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
             }
           }
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float p0 = s[nt][2 * r], p1 = s[nt][2 * r + 1];
-            uint32_t hi, lo;
-            if constexpr (!E4M3) {
-              hi = pack_bf16(p0, p1);
-              lo = pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
-            } else {
-              hi = pack_f16x2(p0, p1);
-              const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              lo = pack_f16x2(p0 - b.x, p1 - b.y);
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float p0 = s[nt][h][2 * r], p1 = s[nt][h][2 * r + 1];
+              uint32_t hi, lo;
+              if constexpr (!E4M3) {
+                hi = pack_bf16(p0, p1);
+                lo = pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
+              } else {
+                hi = pack_f16x2(p0, p1);
+                const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                lo = pack_f16x2(p0 - b.x, p1 - b.y);
+              }
+              ph[nt][h][r] = transpose8x8(hi);
+              pl[nt][h][r] = transpose8x8(lo);
             }
-            ph[nt][r] = transpose8x8(hi);
-            pl[nt][r] = transpose8x8(lo);
-          }
         }
         // V^T fragments of tile i
         auto frag = [&](int i, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3,
@@ -907,86 +1059,100 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           }
         };
         constexpr int D = E4M3 ? 2 : 1;
-        // a weight of 0 does not hide an infinite or NaN value from a row
-        // that does not attend it: such keys go row by row
-        bool apart = false;
-        if (rpb > 1 && k0 + kPaUnit > common) {
-          bool odd = false;
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+        for (int h = 0; h < H; ++h) {
+          const int kh0 = k0 + 16 * h;
+          if constexpr (RING) {
 #pragma unroll
-            for (int q = 0; q < VW; ++q) {
-              const uint32_t v = vr[r][q];
-              if constexpr (!E4M3)
-                odd |= (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
-              else
-                odd |= ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int q = 0; q < VP; ++q) {
+                const uint8_t* p = sv + (16 * h + (r & 1) + 8 * (r >> 1)) * RB + q * 128;
+                if constexpr (VB == 16) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(p);
+                  vr[r][4 * q] = v.x;
+                  vr[r][4 * q + 1] = v.y;
+                  vr[r][4 * q + 2] = v.z;
+                  vr[r][4 * q + 3] = v.w;
+                } else {
+                  const uint2 v = *reinterpret_cast<const uint2*>(p);
+                  vr[r][0] = v.x;
+                  vr[r][1] = v.y;
+                }
+              }
+            if (h == H - 1) {
+              __syncwarp();  // the stage is read: refill it
+              request(st);
             }
-          apart = __any_sync(0xffffffffu, odd);
-        }
-        if (!apart) {
+            // behind the group's keys the stage holds an earlier unit's values
+            if ((bad >> h & 1) || kh0 + 16 > sg.keys) {
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            uint32_t f[4];
-            frag(i, vr[0][i / D], vr[1][i / D], vr[2][i / D], vr[3][i / D], f);
+              for (int r = 0; r < 4; ++r)
+                if ((bad >> h & 1) || kh0 + 2 * c + (r & 1) + 8 * (r >> 1) >= sg.keys) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<!E4M3>(acc[nt][i], f[0], f[1], f[2], f[3], ph[nt][0], ph[nt][1]);
-              mma16816<!E4M3>(acc[nt][i], f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
+                  for (int q = 0; q < VW; ++q) vr[r][q] = 0;
+                }
             }
           }
-        } else {
-          for (int j = 0; j < rpb; ++j) {
-            const int row = sg.row + j;
-            const RowKeys rj = row_keys(a, row);
-            if (row >= a.T || row / rpb != sg.row / rpb || rj.req != req) break;
-            const int at = k0 + 2 * c, keys = rj.keys;
-            const bool on[4] = {at < keys, at + 1 < keys, at + 8 < keys, at + 9 < keys};
+          // a weight of 0 does not hide an infinite or NaN value from a row
+          // that does not attend it: such keys go row by row
+          bool apart = false;
+          if (rpb > 1 && kh0 + 16 > common) {
+            bool odd = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int q = 0; q < VW; ++q) {
+                const uint32_t v = vr[r][q];
+                if constexpr (!E4M3)
+                  odd |= (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
+                else
+                  odd |= ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              }
+            apart = __any_sync(0xffffffffu, odd);
+          }
+          if (!apart) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
               uint32_t f[4];
-              frag(i, on[0] ? vr[0][i / D] : 0, on[1] ? vr[1][i / D] : 0,
-                   on[2] ? vr[2][i / D] : 0, on[3] ? vr[3][i / D] : 0, f);
+              frag(i, vr[0][i / D], vr[1][i / D], vr[2][i / D], vr[3][i / D], f);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                float t[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<!E4M3>(t, f[0], f[1], f[2], f[3], ph[nt][0], ph[nt][1]);
-                mma16816<!E4M3>(t, f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
+                mma16816<!E4M3>(acc[nt][i], f[0], f[1], f[2], f[3], ph[nt][h][0], ph[nt][h][1]);
+                mma16816<!E4M3>(acc[nt][i], f[0], f[1], f[2], f[3], pl[nt][h][0], pl[nt][h][1]);
+              }
+            }
+          } else {
+#pragma unroll 1
+            for (int j = 0; j < rpb; ++j) {
+              const int row = sg.row + j;
+              const RowKeys rj = row_keys(a, row);
+              if (row >= a.T || row / rpb != sg.row / rpb || rj.req != sg.req) break;
+              const int at = kh0 + 2 * c, keys = rj.keys;
+              const bool on[4] = {at < keys, at + 1 < keys, at + 8 < keys, at + 9 < keys};
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if ((nt * 8 + 2 * c + (k & 1)) / G == j) acc[nt][i][k] += t[k];
+              for (int i = 0; i < MT; ++i) {
+                uint32_t f[4];
+                frag(i, on[0] ? vr[0][i / D] : 0, on[1] ? vr[1][i / D] : 0,
+                     on[2] ? vr[2][i / D] : 0, on[3] ? vr[3][i / D] : 0, f);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float t[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma16816<!E4M3>(t, f[0], f[1], f[2], f[3], ph[nt][h][0], ph[nt][h][1]);
+                  mma16816<!E4M3>(t, f[0], f[1], f[2], f[3], pl[nt][h][0], pl[nt][h][1]);
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    if ((nt * 8 + 2 * c + (k & 1)) / G == j) acc[nt][i][k] += t[k];
+                }
               }
             }
           }
         }
-        if (more_u) load_v(u + kPaWarps, pg);
+        if (!RING && more_u) load_v(u + kPaWarps, pg);
       }
-      // the next segment's first unit is on its way while this one's states
-      // are merged
-      const PaSeg done = sg;
-      const long long x0 = x;
-      x += sg.u1 - sg.u0;
-      const bool more = x < x_end;
-      if (more) {
-        sg.u0 = 0;
-        if (++sg.kh == nkv) {
-          sg.kh = 0;
-          unsigned hit = __ballot_sync(0xffffffffu, len_l > 0 && rb + lane > sg.row);
-          while (!hit) {  // there is one: x < total
-            rb += 32;
-            rk = row_keys(a, rb + lane);
-            len_l = lead_keys(rk.keys, rk.req, rpb);
-            hit = __ballot_sync(0xffffffffu, len_l > 0);
-          }
-          sg.row = rb + __ffs(hit) - 1;
-          sg.keys = __shfl_sync(0xffffffffu, len_l, sg.row - rb);
-          req = __shfl_sync(0xffffffffu, rk.req, sg.row - rb);
-          sg.units = units_of(sg.keys);
-        }
-        sg.u1 = (int)min((long long)sg.units, x_end - x);
-        segment();
-        page = page_of(warp);
-      }
+      const long long x0 = at.x;
+      const bool more = advance(at);
+      if (!RING && more) page = page_of(warp);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1000,7 +1166,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
       for (int half = kPaWarps / 2; half > 0; half >>= 1) {
         __syncthreads();
         if (warp >= half && warp < 2 * half) {
-          float4* d = s_acc[warp - half] + lane;
+          float4* d = s_acc + (warp - half) * (NT * MT * 32) + lane;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -1017,15 +1183,16 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           }
         }
         __syncthreads();
-        if (half == kPaWarps / 2) {
-          loaded = more && warp < sg.u1;
+        if (!RING && half == kPaWarps / 2) {
+          // the next segment's first unit, while the states are merged
+          loaded = more && warp < at.sg.u1;
           if (loaded) {
             load_k(warp, page);
             load_v(warp, page);
           }
         }
         if (warp < half) {
-          const float4* d = s_acc[warp] + lane;
+          const float4* d = s_acc + warp * (NT * MT * 32) + lane;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float f0[2], f1[2];
@@ -1050,10 +1217,10 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           }
         }
       }
-      const bool whole = done.u0 == 0 && done.u1 == done.units;
+      const bool whole = sg.u0 == 0 && sg.u1 == sg.units;
       if (warp == 0) {
-        const float sv = E4M3 ? a.kv.v_scale[done.kh] : 1.f;
-        const size_t part = 2 * (size_t)w + (done.u0 == 0 ? 1 : 0);
+        const float sv = E4M3 ? a.kv.v_scale[sg.kh] : 1.f;
+        const size_t part = 2 * (size_t)w + (sg.u0 == 0 ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1062,7 +1229,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
             if (n >= cols) continue;
             const float scale = whole ? sv / l[nt][i] : sv;
             float* po = ws.o + (part * cols + n) * HD;
-            uint16_t* out = a.out + ((size_t)(done.row + n / G) * a.nq + done.kh * G + n % G) * HD;
+            uint16_t* out = a.out + ((size_t)(sg.row + n / G) * a.nq + sg.kh * G + n % G) * HD;
             if (!whole && g == 0)
               ws.ml[part * cols + n] = make_float2(m[nt][i], lim[nt][i] ? l[nt][i] : -1.f);
             if (lim[nt][i] == 0) continue;  // no such row
@@ -1081,11 +1248,11 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
             }
           }
       }
-      if (done.u0 == 0) {
+      if (sg.u0 == 0) {
         const int4 d = whole ? make_int4(-1, 0, 0, 0)
-                             : make_int4(w, (int)((x0 + done.units - 1) / per), done.row, done.kh);
+                             : make_int4(w, (int)((x0 + sg.units - 1) / per), sg.row, sg.kh);
         if (by_row) {
-          if (tid == 0) ws.desc[done.row * nkv + done.kh] = d;
+          if (tid == 0) ws.desc[sg.row * nkv + sg.kh] = d;
         } else if (!whole) {
           my_desc = d;
         }
@@ -1217,28 +1384,34 @@ namespace {
 
 using AttnKernel = void (*)(PagedAttnArgs, PaWork, int);
 
-AttnKernel attn_kernel(int hd, bool e4m3, int G, int* id) {
+AttnKernel attn_kernel(int hd, bool e4m3, int G, int* id, size_t* smem) {
   static const AttnKernel k[8] = {
       k_paged_attn<64, false, 1>,  k_paged_attn<64, false, 2>,
       k_paged_attn<64, true, 1>,   k_paged_attn<64, true, 2>,
       k_paged_attn<128, false, 1>, k_paged_attn<128, false, 2>,
       k_paged_attn<128, true, 1>,  k_paged_attn<128, true, 2>};
-  *id = (hd == 128 ? 4 : 0) + (e4m3 ? 2 : 0) + (G > 8 ? 1 : 0);
+  const int nt = G > 8 ? 2 : 1, rb = hd * (e4m3 ? 1 : 2);
+  *id = (hd == 128 ? 4 : 0) + (e4m3 ? 2 : 0) + nt - 1;
+  // the warps' rings and two warps' accumulators
+  *smem = (e4m3 ? (size_t)kPaWarps * kPaStages * 2 * 16 * pa_halves(e4m3) * rb : 0) +
+          (size_t)kPaWarps / 2 * nt * (hd / 16) * 512;
   return k[*id];
 }
 
 constexpr int kPaMaxCtas = 1024;  // CTAs of a launch (workspace size)
 
 // CTAs that fill the current device; 0 on a CUDA error.
-int attn_ctas(AttnKernel k, int id) {
+int attn_ctas(AttnKernel k, int id, size_t smem) {
   static PerDevice known[8];
   std::atomic<int>& slot = known[id].here();
   int n = slot.load(std::memory_order_relaxed);
   if (!n) {
     int dev = 0, sms = 0, per_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kPaThreads, 0) != cudaSuccess)
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kPaThreads, smem) != cudaSuccess)
       return 0;
     n = sms * per_sm < kPaMaxCtas ? sms * per_sm : kPaMaxCtas;
     slot.store(n, std::memory_order_relaxed);
@@ -1261,14 +1434,16 @@ size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
   int id;
-  const AttnKernel k = attn_kernel(a.kv.hd, e4m3, G, &id);
-  const int full = attn_ctas(k, id);
+  size_t smem;
+  const AttnKernel k = attn_kernel(a.kv.hd, e4m3, G, &id, &smem);
+  const int full = attn_ctas(k, id, smem);
   if (full < 1) return SLX_ERR_CUDA;
   // no more CTAs than steps (a unit per warp) the rows could fill
   const long long segs = (long long)a.T * nkv;
   int grid = full;
   if (segs < (long long)full * kPaWarps) {
-    const long long row_units = (long long)a.max_pages * (a.kv.page_size / kPaUnit);
+    const int ku = 16 * pa_halves(e4m3);
+    const long long row_units = ((long long)a.max_pages * a.kv.page_size + ku - 1) / ku;
     const long long steps = (segs * row_units + kPaWarps - 1) / kPaWarps;
     if (steps < full) grid = (int)steps;
   }
@@ -1278,7 +1453,7 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   ws.desc = reinterpret_cast<int4*>(p);
   ws.o = reinterpret_cast<float*>(p + kPaMaxCtas * sizeof(int4));
   ws.ml = reinterpret_cast<float2*>(ws.o + (size_t)kPaMaxCtas * 2 * cols * a.kv.hd);
-  if (launch_k(k, dim3(grid), dim3(kPaThreads), 0, s, a, ws, rpb) != cudaSuccess)
+  if (launch_k(k, dim3(grid), dim3(kPaThreads), smem, s, a, ws, rpb) != cudaSuccess)
     return SLX_ERR_CUDA;
   // one CTA per column while they fit the device about twice over
   const unsigned n = (unsigned)(segs <= grid ? segs : grid);
