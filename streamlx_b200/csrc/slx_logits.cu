@@ -301,22 +301,10 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
           touched = (lo.x != 0) | (lo.y != 0) << 1 | (lo.z != 0) << 2 | (lo.w != 0) << 3 |
                     (hi.x != 0) << 4 | (hi.y != 0) << 5 | (hi.z != 0) << 6 | (hi.w != 0) << 7;
       }
-      if (const uint32_t list = touched & ok[v]; __any_sync(0xffffffffu, list)) {
-        int at = __popc(list);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += u;
-        }
-        int base = 0;
-        if (lane == 31) base = atomicAdd(&s_n, at);
-        at += __shfl_sync(0xffffffffu, base, 31) - __popc(list);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (list >> j & 1) {
-            if (at < kLogitList) s_list[at] = (uint16_t)(q * 8 + j);
-            ++at;
-          }
+      if (uint32_t list = touched & ok[v]) {
+        int at = atomicAdd(&s_n, __popc(list));
+        for (; list; list &= list - 1, ++at)
+          if (at < kLogitList) s_list[at] = (uint16_t)(q * 8 + __ffs(list) - 1);
       }
       if (ok[v]) first = min(first, id + __ffs(ok[v]) - 1);
       if (ok[v] != 0xffu) raw[v].mask(ok[v]);

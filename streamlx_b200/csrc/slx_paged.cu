@@ -432,6 +432,7 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = 32 * kPaWarps;
 constexpr int kPaStages = 2;  // of a warp's ring
+constexpr int kPaSwitch = 8;
 // 16-key halves of a unit: as many bytes in flight either way
 constexpr int pa_halves(bool e4m3) { return e4m3 ? 2 : 1; }
 
@@ -508,18 +509,18 @@ SLX_DEV int lead_keys(int n, int r, int rpb) {
   const int lane = threadIdx.x & 31;
   const int before = __shfl_up_sync(0xffffffffu, r, 1);
   const bool first = lane % rpb == 0 || before != r;
-  bool same = true;
+  const unsigned starts = __ballot_sync(0xffffffffu, first);
+  const unsigned behind = lane == 31 ? 0u : starts >> (lane + 1);
+  const int end = behind ? lane + __ffs(behind) : 32;  // of this lane's group
   int most = n;
-  for (int d = 1; d < rpb; ++d) {
-    const int rd = __shfl_down_sync(0xffffffffu, r, d);
-    const int nd = __shfl_down_sync(0xffffffffu, n, d);
-    same = same && lane % rpb + d < rpb && rd == r;
-    if (same) most = max(most, nd);
+  for (int d = 1; d < rpb; d <<= 1) {
+    const int v = __shfl_down_sync(0xffffffffu, most, d);
+    if (lane + d < end) most = max(most, v);
   }
   return first ? most : 0;
 }
 
-// Sum of 0 <= n <= 2^27 over a warp.
+// Sum of 0 <= n < 2^28 over a warp.
 SLX_DEV long long warp_sum(int n) {
   return (long long)__reduce_add_sync(0xffffffffu, (unsigned)n & 0xffffu) +
          ((long long)__reduce_add_sync(0xffffffffu, (unsigned)n >> 16) << 16);
@@ -564,7 +565,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   pdl_launch_dependents();
   pdl_wait_primary();
   auto units_of = [](int keys) { return (int)(((unsigned)keys + kPaUnit - 1) / kPaUnit); };
-  // units before each of 128 runs of `run` tiles of 32 rows
+  auto weight_of = [&](int keys) { return keys ? units_of(keys) + kPaSwitch : 0; };
+  // weights before each of 128 runs of `run` tiles of 32 rows
   const int tiles = (a.T + 31) / 32, run = (tiles + kPaThreads - 1) / kPaThreads;
   RowKeys rk;                             // of row rb + lane
   int len_l = 0;                          // keys of the group it leads
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   if (tiles == 1) {
     rk = row_keys(a, lane);
     len_l = lead_keys(rk.keys, rk.req, rpb);
-    total = warp_sum(units_of(len_l)) * nkv;
+    total = warp_sum(weight_of(len_l)) * nkv;
   } else {
     s_pre[tid + 1] = 0;
     __syncthreads();
@@ -583,7 +585,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
       for (int j = 0; j < B; ++j) r[j] = row_keys(a, (i0 + j) * 32 + lane);
 #pragma unroll
       for (int j = 0; j < B; ++j) {
-        const long long v = warp_sum(units_of(lead_keys(r[j].keys, r[j].req, rpb)));
+        const long long v = warp_sum(weight_of(lead_keys(r[j].keys, r[j].req, rpb)));
         if (lane == 0 && i0 + j < tiles)
           atomicAdd(reinterpret_cast<unsigned long long*>(&s_pre[(i0 + j) / run + 1]),
                     (unsigned long long)v);
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
     PaSeg sg;
     int rb = 0;
     {
-      // the group unit x is in: its run of tiles, then tile by tile
+      // the segment x is in: its run of tiles, then tile by tile
       long long before = 0;
       if (tiles > 1) {
         if (s_pre[tid] * nkv <= x && x < s_pre[tid + 1] * nkv) s_run = tid;
@@ -629,42 +631,50 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           rk = row_keys(a, rb + lane);
           len_l = lead_keys(rk.keys, rk.req, rpb);
         }
-        const int n = units_of(len_l);
-        long long v = n;
+        const int n = weight_of(len_l);
+        const long long all = warp_sum(n);
+        if (x >= before + all * nkv) {
+          before += all * nkv;
+          continue;
+        }
+        // the row whose weights (times nkv) reach beyond x
+        auto find = [&](auto v, auto in) {
+          const auto own = v;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long u = __shfl_up_sync(0xffffffffu, v, o);
-          if (lane >= o) v += u;
-        }
-        const bool here = before + (v - n) * nkv <= x && x < before + v * nkv;
-        const unsigned hit = __ballot_sync(0xffffffffu, here);
-        if (hit) {
-          const int i = __ffs(hit) - 1;
+          for (int o = 1; o < 32; o <<= 1) {
+            const auto u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+          }
+          const int i = __ffs(__ballot_sync(0xffffffffu, v > in)) - 1;
           sg.row = rb + i;
-          before += (__shfl_sync(0xffffffffu, v, i) - __shfl_sync(0xffffffffu, n, i)) * nkv;
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, v, 31) * nkv;
+          before += (long long)__shfl_sync(0xffffffffu, v - own, i) * nkv;
+          return i;
+        };
+        const long long in = x - before < 0x7fffffff ? (unsigned)(x - before) / (unsigned)nkv : (x - before) / nkv;
+        const int i = all < 0x7fffffff ? find(n, (int)in) : find((long long)n, in);
+        sg.keys = __shfl_sync(0xffffffffu, len_l, i);
+        sg.req = __shfl_sync(0xffffffffu, rk.req, i);
+        break;
       }
-      sg.keys = __shfl_sync(0xffffffffu, len_l, sg.row - rb);
-      sg.req = __shfl_sync(0xffffffffu, rk.req, sg.row - rb);
       sg.units = units_of(sg.keys);
+      const int weight = sg.units + kPaSwitch;
       const long long in = x - before;
-      sg.kh = in < 0x7fffffff ? (int)((unsigned)in / (unsigned)sg.units)
-                              : (int)(in / sg.units);
-      sg.u0 = (int)(in - (long long)sg.kh * sg.units);
-      sg.u1 = (int)min((long long)sg.units, sg.u0 + (x_end - x));
+      sg.kh = in < 0x7fffffff ? (int)((unsigned)in / (unsigned)weight) : (int)(in / weight);
+      before += (long long)sg.kh * weight + kPaSwitch;  // of the segment's first unit
+      sg.u0 = (int)max(x - before, 0LL);
+      sg.u1 = (int)max(min((long long)sg.units, x_end - before), 0LL);
+      x = before;
     }
     const size_t page_bytes = (size_t)2 * nkv * ps * RB, v_off = (size_t)nkv * ps * RB;
     // a place in the CTA's segments: the rows of tile rb and x as above
     struct Place {
       PaSeg sg;
       int rb, len, req;  // len, req: of row rb + lane
-      long long x;
+      long long x;       // the place of the segment's first unit
     };
     // to the next segment; false behind the last
     auto advance = [&](Place& p) {
-      p.x += p.sg.u1 - p.sg.u0;
+      p.x += p.sg.units + kPaSwitch;
       if (p.x >= x_end) return false;
       p.sg.u0 = 0;
       if (++p.sg.kh == nkv) {
@@ -818,7 +828,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
 #pragma unroll
       for (int i = 0; i < S; ++i) request(i);
     }
-    while (true) {
+    // (a CTA whose share ends before a first unit computes nothing)
+    while (at.sg.u1 > at.sg.u0) {
       sg = at.sg;
       int u = sg.u0 + warp;
       // columns n of the MMAs: row n / G of the group, q head n % G
@@ -1280,16 +1291,16 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
 }
 
 // Parts of one split (group, kv head) added in the order of the keys, a thread
-// per four dims of a column and NG parts side by side; each thread requests
-// eight parts before it uses one.  COL: one column per CTA (few segments of
-// many parts), else all columns (many segments of a few parts, and most CTAs
-// find nothing to do).
-constexpr int kJoinThreads = 512;
-constexpr int kJoinBatch = 8;
+// per four dims of a column and NG parts side by side; each thread requests a
+// batch of parts before it uses one.  COL: one column per CTA (few segments of
+// many parts), else all columns in a smaller CTA (many segments of a few
+// parts, and most CTAs find nothing to do).
+constexpr int kJoinThreads = 512;   // at most
 
 template <int HD, bool COL>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedAttnArgs a,
                                                              const PaWork ws, int rpb) {
+  constexpr int kJoinBatch = COL ? 8 : 4;
   __shared__ __align__(16) float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   pdl_launch_dependents();
@@ -1299,7 +1310,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedAttnArgs
   constexpr int TP = HD / 4;                 // threads per column
   const int G = a.nq / a.kv.n_kv, cols = rpb * G;
   const int width = COL ? TP : cols * TP;    // threads per part
-  const int NG = kJoinThreads / width;       // parts side by side
+  const int NG = blockDim.x / width;         // parts side by side
   const int tid = threadIdx.x, q = tid / width;
   const int n = COL ? blockIdx.y : tid % width / TP, d4 = tid % TP * 4;
   const int parts = d.y - d.x + 1;
@@ -1460,7 +1471,9 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const bool col = n * (unsigned)cols <= 1024;
   auto j = a.kv.hd == 128 ? (col ? k_paged_join<128, true> : k_paged_join<128, false>)
                           : (col ? k_paged_join<64, true> : k_paged_join<64, false>);
-  return launch_chained(j, dim3(n, col ? cols : 1), dim3(kJoinThreads), 0, s, a, ws, rpb) ==
+  const int width = cols * (a.kv.hd / 4);
+  const int threads = col || 2 * width > kJoinThreads ? kJoinThreads : 2 * width;
+  return launch_chained(j, dim3(n, col ? cols : 1), dim3(threads), 0, s, a, ws, rpb) ==
                  cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
 }
 
