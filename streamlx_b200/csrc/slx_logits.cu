@@ -116,6 +116,22 @@ struct Raw8<float> {
   SLX_DEV void store1(int j, float* p) const { *p = f[j]; }
 };
 
+// Order of the picks as integers: greater values have greater keys.
+SLX_DEV uint64_t pick_key(double v) {
+  const long long b = __double_as_longlong(v + 0.0);  // -0 is 0
+  return (uint64_t)(b < 0 ? ~b : b ^ (long long)0x8000000000000000ull);
+}
+
+// The greatest key of a warp's lanes and its lowest id, in every lane.
+SLX_DEV void warp_best(uint64_t& key, int& id) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+  const bool a = (uint32_t)(key >> 32) == hi;
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, a ? (uint32_t)key : 0u);
+  id = (int)__reduce_min_sync(0xffffffffu,
+                              a && (uint32_t)key == lo ? (uint32_t)id : 0x7fffffffu);
+  key = (uint64_t)hi << 32 | lo;
+}
+
 // A cluster of 8 CTAs per row; runs of 32 vectors of eight ids (a warp's
 // load) go round the CTAs, because the ids that rules touch crowd at the
 // vocabulary's start and the cluster waits for its slowest CTA.  Every thread
@@ -134,10 +150,8 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
   extern __shared__ __align__(16) uint32_t s_word[];
   __shared__ uint16_t s_list[kLogitList];
   __shared__ int s_n;
-  __shared__ double s_v[kLogitThreads / 32];
-  __shared__ int s_i[kLogitThreads / 32];
-  __shared__ double c_v[kLogitCluster];
-  __shared__ int c_i[kLogitCluster];
+  __shared__ uint64_t s_key[kLogitThreads / 32], c_key[kLogitCluster];
+  __shared__ int s_id[kLogitThreads / 32], c_id[kLogitCluster];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank();
   const int row = blockIdx.x / kLogitCluster;
@@ -375,33 +389,31 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
   // an allowed id whose logit is -inf (or NaN) is picked only if all are
   if (first != 0x7fffffff) best.take(-INFINITY, first);
   if (plain_i != 0x7fffffff) best.take((double)plain, plain_i);
-  auto over = [&](int lanes) {  // of the first `lanes` lanes (a power of two)
-    for (int o = lanes / 2; o > 0; o >>= 1) {
-      const double v = __shfl_xor_sync(0xffffffffu, best.v, o);
-      const int i = __shfl_xor_sync(0xffffffffu, best.i, o);
-      best.take(v, i);
-    }
-  };
-  over(32);
+  // (key 0 is below every value's)
+  uint64_t key = best.i == 0x7fffffff ? 0 : pick_key(best.v);
+  int id = best.i;
+  warp_best(key, id);
   if (lane == 0) {
-    s_v[warp] = best.v;
-    s_i[warp] = best.i;
+    s_key[warp] = key;
+    s_id[warp] = id;
   }
   __syncthreads();
   if (warp == 0) {
     constexpr int W = kLogitThreads / 32;
-    best = {s_v[lane % W], s_i[lane % W]};
-    over(W);
+    key = s_key[lane % W];
+    id = s_id[lane % W];
+    warp_best(key, id);
     if (lane == 0) {
-      *cluster.map_shared_rank(&c_v[rank], 0) = best.v;
-      *cluster.map_shared_rank(&c_i[rank], 0) = best.i;
+      *cluster.map_shared_rank(&c_key[rank], 0) = key;
+      *cluster.map_shared_rank(&c_id[rank], 0) = id;
     }
   }
   cluster.sync();
   if (rank == 0 && warp == 0) {
-    best = {c_v[lane % kLogitCluster], c_i[lane % kLogitCluster]};
-    over(kLogitCluster);
-    if (lane == 0) a.pick[row] = best.i < a.V ? best.i : -1;
+    key = c_key[lane % kLogitCluster];
+    id = c_id[lane % kLogitCluster];
+    warp_best(key, id);
+    if (lane == 0) a.pick[row] = id < a.V ? id : -1;
   }
 }
 
