@@ -913,8 +913,9 @@ int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
   if (T < 0 || n_q < 1 || n_q % a.kv.n_kv || n_q / a.kv.n_kv > 16)
     return fail(SLX_ERR_INVALID, "paged_attn: T %d n_q %d n_kv %d (at most 16 q heads a kv head)",
                 T, n_q, a.kv.n_kv);
-  if (n_req < 1 || max_pages < 1 || (long long)max_pages * a.kv.page_size > 0x7fffffffLL)
-    return fail(SLX_ERR_INVALID, "paged_attn: n_req %d max_pages %d", n_req, max_pages);
+  if (n_req < 1 || max_pages < 1 || (long long)max_pages * a.kv.page_size > (1LL << 30))
+    return fail(SLX_ERR_INVALID, "paged_attn: n_req %d max_pages %d (at most 2^30 tokens a request)",
+                n_req, max_pages);
   if (!req && T > n_req)
     return fail(SLX_ERR_INVALID, "paged_attn: T %d rows, %d requests and no req", T, n_req);
   if (T == 0) return SLX_OK;

@@ -169,7 +169,8 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
   // ids 8 k - lead .. + 7, the first and last perhaps not whole
   constexpr int AL = 16 / sizeof(T);
   const int lead = (int)((reinterpret_cast<uintptr_t>(x_row) / sizeof(T)) % AL);
-  const bool same = ((reinterpret_cast<uintptr_t>(x_row) ^ reinterpret_cast<uintptr_t>(o_row)) & 15) == 0;
+  const bool same =
+      ((reinterpret_cast<uintptr_t>(x_row) ^ reinterpret_cast<uintptr_t>(o_row)) & 15) == 0;
   const int n_vec = (int)(((long long)a.V + lead + 7) / 8);
   // this CTA's q-th vector; a thread's next one is `hop` vectors on
   auto vec_at = [&](int q) { return ((q >> 5) * kLogitCluster + rank) * 32 + (q & 31); };

@@ -402,14 +402,14 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // with mma.m16n8k16: M is keys / dims, so no row is padding (tcgen05's
 // smallest M of 64 or 128 heads would be).  The columns are the q heads of
 // one row and, where they leave room, of the rows after it that belong to the
-// same request (a prompt's rows share their keys: see group_of).
+// same request (a prompt's rows share their keys: see lead_keys).
 //
 // The contraction index of an MMA may be permuted on both sides alike; the
 // fragments are chosen so that each is 16 contiguous bytes of a key.
 //   bf16: keys and values go from global memory to fragments without shared
 //   memory, the next unit's into the registers that this one's have just left
-//   (482 us for 256 requests of 6k tokens, 24/4 heads; through the ring below
-//   499).
+//   (478 us for 256 requests of 6k tokens, 24/4 heads, 6.9 TB/s; through the
+//   ring below 499).
 //   e4m3: half the bytes and twice the work per byte.  A unit's keys and its
 //   values are one contiguous block each: every warp has a ring of stages in
 //   shared memory that its first lane fills by bulk copies, some units ahead
@@ -423,16 +423,18 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // exactly; q becomes fp16 times a power of two per head that puts its largest
 // element at 2^12 .. 2^13 (exact down to 2^-26 of it).
 //
-// Work is cut into units of 16 keys of one kv head; every CTA gets the same
-// number of consecutive units of the list (row group, kv head, unit), whatever
-// the rows' lengths.  A (group, kv head) that one CTA covers
-// is written directly, the others leave (max, sum, O) parts that
+// Work is cut into units of one kv head (16 bf16 or 32 e4m3 keys); every CTA
+// gets an equal share of the list (row group, kv head, unit), whatever the
+// rows' lengths.  A segment, the units of one (group, kv head), weighs
+// kPaSwitch units more than it has, about what the change to it costs (64
+// requests of 0 to 4k tokens: 51 us, 59 without).  A segment that one CTA
+// covers is written directly, the others leave (max, sum, O) parts that
 // k_paged_join adds in order.
 
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = 32 * kPaWarps;
 constexpr int kPaStages = 2;  // of a warp's ring
-constexpr int kPaSwitch = 8;
+constexpr int kPaSwitch = 8;  // units
 // 16-key halves of a unit: as many bytes in flight either way
 constexpr int pa_halves(bool e4m3) { return e4m3 ? 2 : 1; }
 
@@ -480,7 +482,6 @@ SLX_DEV void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
       "cvt.rn.f16x2.e4m3x2 %1, u;}"
       : "=r"(lo), "=r"(hi) : "r"(w));
 }
-
 
 // Row t's request and the keys it attends: pos + 1, 0 for an idle row or one
 // out of range.  (Both are read at once: rows are read in batches.)
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
     __syncthreads();
     total = s_pre[kPaThreads] * nkv;
   }
-  // units per CTA: a multiple of the warps (a step is one unit per warp)
+  // weight per CTA: a multiple of the warps (a step is one unit per warp)
   long long per = total < 0x7fffffff - nw ? ((unsigned)total + nw - 1) / (unsigned)nw
                                           : (total + nw - 1) / nw;
   per = (per + kPaWarps - 1) / kPaWarps * kPaWarps;
@@ -650,7 +651,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           before += (long long)__shfl_sync(0xffffffffu, v - own, i) * nkv;
           return i;
         };
-        const long long in = x - before < 0x7fffffff ? (unsigned)(x - before) / (unsigned)nkv : (x - before) / nkv;
+        const long long in = x - before < 0x7fffffff ? (unsigned)(x - before) / (unsigned)nkv
+                                                     : (x - before) / nkv;
         const int i = all < 0x7fffffff ? find(n, (int)in) : find((long long)n, in);
         sg.keys = __shfl_sync(0xffffffffu, len_l, i);
         sg.req = __shfl_sync(0xffffffffu, rk.req, i);
@@ -843,9 +845,12 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
         const int n = nt * 8 + g;
         int row = sg.row, keys = n < cols ? sg.keys : 0;
         if (rpb > 1) {
+          // the group ends before its first row of another request or block
           row += n / G;
           const RowKeys r = row_keys(a, row);
-          keys = n < cols && row / rpb == sg.row / rpb && r.req == sg.req ? r.keys : 0;
+          const bool on = row < a.T && row / rpb == sg.row / rpb && r.req == sg.req;
+          const int rows = __reduce_min_sync(0xffffffffu, on ? rpb : n / G);
+          keys = n < cols && n / G < rows ? r.keys : 0;
         }
         lim[nt][0] = __shfl_sync(0xffffffffu, keys, 8 * c);
         lim[nt][1] = __shfl_sync(0xffffffffu, keys, 8 * c + 4);

@@ -216,6 +216,76 @@ def test_bias_entries_limit():
     assert run(c, "new")[2] == L.SLX_ERR_OUT_OF_RANGE
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [999, 4104])
+def test_rows_at_any_alignment(V, dtype):
+    """Logits, output and history whose rows start anywhere."""
+    c = case(5, V, dtype, 37, 11, True, seed=V)
+    base, _, _ = run(c, "new")
+    for a, b in ((0, 0), (1, 1), (1, 0), (0, 3), (5, 2)):
+        def put(t, off):
+            buf = torch.empty(t.numel() + off, dtype=t.dtype, device="cuda")
+            v = buf[off:].view(t.shape)
+            v.copy_(t)
+            return v
+        x, h = put(c["x"], a), put(c["history"], a + b)
+        out = put(torch.zeros_like(c["x"]), b)
+        pick = ops.process_logits(
+            x, h, c["n_prompt"].cuda(), c["n_history"].cuda(),
+            repetition=c["rep"].cuda(), frequency=c["freq"].cuda(),
+            presence=c["pres"].cuda(), bias=tuple(t.cuda() for t in c["bias"]),
+            mask=c["mask"].cuda(), out=out)
+        want, picks = P.logits(c["x"], c["history"], c["n_prompt"],
+                               c["n_history"], c["rep"], c["freq"], c["pres"],
+                               c["bias"], c["mask"])
+        assert pick.tolist() == picks == base
+        fin = torch.isfinite(want)
+        y = out.cpu().double()
+        assert torch.equal(torch.isfinite(y), fin)
+        half = torch.finfo(dtype).eps / 2 + 2.0 ** -23
+        assert ((y - want)[fin].abs() <= half * want[fin].abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_most_ids_touched(dtype):
+    """A history that names most of the vocabulary: more ids than a pass
+    lists."""
+    V, n = 151936, 131072
+    g = torch.Generator().manual_seed(10)
+    ids = torch.randperm(V, generator=g)[:n].to(torch.int32)[None]
+    x = (torch.randn(1, V, generator=g) * 2.5).to(dtype)
+    rep, freq = torch.tensor([1.3]), torch.tensor([0.25])
+    c = dict(case(1, V, dtype, 0, 0, False), x=x, history=ids,
+             n_prompt=torch.tensor([n // 2], dtype=torch.int32),
+             n_history=torch.tensor([n], dtype=torch.int32), rep=rep,
+             freq=freq)
+    got, y, st = run(c, "new")
+    want = x[0].double()
+    at = ids[0].long()
+    v = want[at]
+    want[at] = torch.where(v > 0, v / rep.double(), v * rep.double())
+    want[at[n // 2:]] -= freq.double()
+    assert st == 0 and got == [int(want.argmax())]
+    half = torch.finfo(dtype).eps / 2 + 2.0 ** -23
+    assert ((y[0].double() - want).abs() <= half * want.abs()).all()
+
+
+def test_one_id_all_along():
+    """The longest history, every entry the same id."""
+    n = 262143
+    x = torch.zeros(1, 100, dtype=F32)
+    c = dict(case(1, 100, F32, 0, 0, False), x=x,
+             history=torch.full((1, n), 7, dtype=torch.int32),
+             n_history=torch.tensor([n], dtype=torch.int32),
+             freq=torch.tensor([0.5]), pres=torch.tensor([1.0]),
+             bias=(torch.tensor([7, 7], dtype=torch.int32),
+                   torch.tensor([9.0, 2.5]),
+                   torch.tensor([0, 2], dtype=torch.int32)))
+    got, y, st = run(c, "new")
+    assert st == 0 and got == [0]
+    assert float(y[0, 7]) == -0.5 * n - 1.0 + 2.5
+
+
 def test_without_pick_and_empty():
     c = case(2, 500, BF, 30, 5, True, seed=8)
     _, y, _ = run(c, "new")

@@ -65,7 +65,8 @@ def test_bad_pages(fields, code):
 
 @pytest.mark.parametrize("kw", [
     dict(T=-1), dict(n_q=15), dict(n_q=0), dict(n_q=34), dict(n_req=0),
-    dict(n_req=2), dict(max_pages=0), dict(max_pages=1 << 28), dict(q=None),
+    dict(n_req=2), dict(max_pages=0), dict(max_pages=1 << 28),
+    dict(max_pages=(1 << 26) + 1), dict(q=None),
     dict(q=PTR + 8), dict(q_stride=16 * 128 - 8), dict(q_stride=16 * 128 + 4),
     dict(table=None), dict(pos=None), dict(out=None), dict(out=PTR + 2)])
 def test_bad_attention(kw):

@@ -1,6 +1,10 @@
 """Batched decode over a paged KV cache against plain 64-bit restatements
 (tests/paged_cases.py): the step's plan, the append and the attention."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -141,6 +145,18 @@ def test_attention_prompt_rows_hide_later_values(nq, nkv, hd, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 8, 64), (4, 2, 128), (9, 3, 64)])
+def test_attention_rows_of_requests_in_turn(nq, nkv, hd, dtype):
+    """Rows of two requests alternating, the later ones longer: rows that
+    follow a row of another request are not the first one's group."""
+    lens = [300, 280]
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=16)
+    req = [0, 1] * 8 + [0, 0, 1, 0, 0, 0, 1, 1]
+    pos = [int(p) for p in np.linspace(3, 270, 24)]
+    check_attention(queries(24, nq, hd), host, dev, req, pos)
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
 def test_attention_long_prompt_rows(dtype):
     """A chunk of rows behind a long prefix: groups split over CTAs."""
     lens = [6000, 333]
@@ -197,20 +213,29 @@ def test_attention_infinite_and_nan_keys():
     assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
 
 
-def test_attention_bad_indices():
+@pytest.mark.parametrize("dtype,hd", [(BF, 128), (E4, 128), (E4, 64)])
+def test_attention_bad_indices(dtype, hd):
     """A page, request or position out of range sets the status, is not
     followed, and leaves the other rows right."""
     lens = [40, 50, 60]
-    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=10)
+    host, dev = dev_cache(lens, 2, hd, 16, dtype, seed=10)
     pages, sc, table = dev
-    q = queries(3, 16, 128)
+    q = queries(3, 16, hd)
     good = check_attention(q, host, dev, None, [39, 49, 59])
     for bad in (-1, pages.shape[0], 2 ** 31 - 1):
-        t = table.clone()
-        t[1, 2] = bad
-        out, st = run_attention(q, (pages, sc, t), None, [39, 49, 59])
-        assert st == L.SLX_ERR_OUT_OF_RANGE
-        assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+        for col in range(4):
+            t = table.clone()
+            t[1, col] = bad
+            out, st = run_attention(q, (pages, sc, t), None, [39, 49, 59])
+            assert st == L.SLX_ERR_OUT_OF_RANGE
+            assert torch.equal(out[0], good[0])
+            assert torch.equal(out[2], good[2])
+            # the page's keys and values read as zeros
+            zero = host[0].float()
+            zero[int(host[2][1, col])] = 0
+            want, bound = P.attention(q[1:2], zero.to(dtype), host[1],
+                                      host[2], [1], [49], 16, hd ** -0.5)
+            assert ((out[1:2].double() - want).abs() <= bound).all()
     cap = table.shape[1] * 16
     for req, pos in (([0, 3, 2], [39, 49, 59]), ([0, -1, 2], [39, 49, 59]),
                      ([0, 1, 2], [39, cap, 59]),
@@ -297,6 +322,110 @@ def test_attention_far_pages():
     want, bound = P.attention(q, small, sc.cpu(), near, [0, 1], [249, 99],
                               page, hd ** -0.5)
     assert st == 0 and ((out.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("T", [1, 33, 2000])
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_all_rows_idle(T, dtype):
+    host, dev = dev_cache([5], 2, 64, 16, dtype, seed=17)
+    out, st = run_attention(queries(T, 4, 64), dev, [0] * T, [-1] * T)
+    assert st == 0 and (out == 0).all()
+    pos = [-1] * T
+    pos[T // 2] = 4
+    check_attention(queries(T, 4, 64), host, dev, [0] * T, pos)
+
+
+def test_attention_many_kv_heads():
+    """More kv heads than a CTA has threads."""
+    lens = [70, 0, 33]
+    host, dev = dev_cache(lens, 200, 64, 16, BF, seed=18)
+    check_attention(queries(3, 200, 64), host, dev, None,
+                    [n - 1 for n in lens])
+
+
+def test_chained_launches():
+    """The step's kernels under programmatic dependent launch, eagerly and in
+    a graph, give the same bits as without."""
+    def step(state):
+        n_new, ln, table, free, nf, qkv, pages, qn, kn, inv, logits = state
+        p = ops.paged_plan(n_new, ln, table, free, nf, 16, 40)
+        q = ops.paged_append(qkv, pages, p.slot, p.pos, 8, qn, kn, EPS, inv)
+        o = ops.paged_attention(q, pages, table, p.pos, req=p.req)
+        pick = ops.process_logits(logits)
+        return [*p, q, o, pick, pages, table]
+
+    def fresh():
+        g = torch.Generator(device="cuda").manual_seed(5)
+        i32 = dict(dtype=torch.int32, device="cuda")
+
+        def rn(*shape):
+            return torch.randn(*shape, generator=g, device="cuda").to(BF)
+        return (torch.tensor([20, 1, 0, 9], **i32),
+                torch.tensor([0, 31, 5, 0], **i32),
+                torch.tensor([[-1] * 6, [0, 1] + [-1] * 4, [2] + [-1] * 5,
+                              [-1] * 6], **i32),
+                torch.arange(3, 43, **i32) % 40, torch.tensor([37], **i32),
+                rn(40, 12 * 64), rn(40, 2, 2, 16, 64), rn(64), rn(64),
+                torch.rand(32, generator=g, device="cuda"), rn(40, 5000))
+
+    want = [t.clone() for t in step(fresh())]
+    prev = L.set_pdl(True)
+    try:
+        s1, s2 = fresh(), fresh()
+        torch.cuda.synchronize()
+        a = step(s1)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            b = step(s2)
+        graph.replay()
+        torch.cuda.synchronize()
+    finally:
+        L.set_pdl(prev)
+    for got in (a, b):
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    ops.check_status(torch.device("cuda", torch.cuda.current_device()))
+
+
+def test_first_calls_in_a_capture():
+    """In a new process, the first call of every operator inside a capture."""
+    code = """
+import sys, torch
+sys.path.insert(0, %r)
+from streamlx_b200 import ops
+i32 = dict(dtype=torch.int32, device='cuda')
+bf = dict(dtype=torch.bfloat16, device='cuda')
+n_new, ln = torch.ones(3, **i32), torch.zeros(3, **i32)
+table = torch.full((3, 4), -1, **i32)
+free, nf = torch.arange(9, **i32), torch.tensor([9], **i32)
+qkv, w = torch.randn(3, 8 * 64, device='cuda').bfloat16(), torch.ones(64, **bf)
+pages = torch.zeros(9, 2, 2, 16, 64, **bf)
+p8 = torch.zeros(9, 2, 2, 16, 64, device='cuda').to(torch.float8_e4m3fn)
+sc, inv = torch.ones(2, 2, device='cuda'), torch.ones(32, device='cuda')
+logits = torch.randn(3, 999, device='cuda')
+torch.cuda.synchronize()
+
+def step():
+    p = ops.paged_plan(n_new, ln, table, free, nf, 16, 3)
+    out = []
+    for pg, s in ((pages, None), (p8, sc)):
+        q = ops.paged_append(qkv, pg, p.slot, p.pos, 4, w, w, 1e-6, inv,
+                             kv_scale=s)
+        out.append(ops.paged_attention(q, pg, table, p.pos, req=p.req,
+                                       kv_scale=s))
+    return out + [ops.process_logits(logits), p.slot]
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = step()
+g.replay()
+b = step()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(a, b))
+print('same')
+""" % os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
 
 
 def test_attention_no_rows_and_grid_limit():
