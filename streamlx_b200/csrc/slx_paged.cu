@@ -500,8 +500,8 @@ SLX_DEV RowKeys row_keys(const PagedAttnArgs& a, int t) {
   return r;
 }
 
-// Rows are taken in aligned blocks of `rpb` (1, 2, 4 or 8: what fits the MMA's
-// columns); within one, consecutive rows of the same request form a group.
+// Rows are taken in aligned blocks of `rpb` (a power of two up to 16: what fits
+// the MMA's columns); within one, consecutive rows of the same request form a group.
 // For a warp over rows t0 .. t0 + 31 (t0 a multiple of 32; n and r its rows'
 // keys and requests): the keys of the group that row t0 + lane leads, 0 if it
 // leads none.
@@ -840,6 +840,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
       int lim[NT][2];    // their keys (0: no such row)
       const float fs = a.scale * 1.4426950408889634f * (E4M3 ? a.kv.k_scale[sg.kh] : 1.f);
       uint4 qv[NT][HD / 32];
+      int rows = rpb;    // of the group
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int n = nt * 8 + g;
@@ -849,7 +850,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
           row += n / G;
           const RowKeys r = row_keys(a, row);
           const bool on = row < a.T && row / rpb == sg.row / rpb && r.req == sg.req;
-          const int rows = __reduce_min_sync(0xffffffffu, on ? rpb : n / G);
+          rows = min(rows, (int)__reduce_min_sync(0xffffffffu, on ? rpb : n / G));
           keys = n < cols && n / G < rows ? r.keys : 0;
         }
         lim[nt][0] = __shfl_sync(0xffffffffu, keys, 8 * c);
@@ -1400,13 +1401,13 @@ namespace {
 
 using AttnKernel = void (*)(PagedAttnArgs, PaWork, int);
 
-AttnKernel attn_kernel(int hd, bool e4m3, int G, int* id, size_t* smem) {
+AttnKernel attn_kernel(int hd, bool e4m3, int nt, int* id, size_t* smem) {
   static const AttnKernel k[8] = {
       k_paged_attn<64, false, 1>,  k_paged_attn<64, false, 2>,
       k_paged_attn<64, true, 1>,   k_paged_attn<64, true, 2>,
       k_paged_attn<128, false, 1>, k_paged_attn<128, false, 2>,
       k_paged_attn<128, true, 1>,  k_paged_attn<128, true, 2>};
-  const int nt = G > 8 ? 2 : 1, rb = hd * (e4m3 ? 1 : 2);
+  const int rb = hd * (e4m3 ? 1 : 2);
   *id = (hd == 128 ? 4 : 0) + (e4m3 ? 2 : 0) + nt - 1;
   // the warps' rings and two warps' accumulators
   *smem = (e4m3 ? (size_t)kPaWarps * kPaStages * 2 * 16 * pa_halves(e4m3) * rb : 0) +
@@ -1435,23 +1436,38 @@ int attn_ctas(AttnKernel k, int id, size_t smem) {
   return n;
 }
 
-// Rows that share a group's MMA columns.
-int attn_rows(int G) { return G == 1 ? 8 : G == 2 ? 4 : G <= 4 ? 2 : 1; }
+// Rows that share a group's MMA columns: as many as fit, a power of two.
+int attn_rows(int G, int nt) {
+  int n = 1;
+  while (2 * n * G <= 8 * nt) n *= 2;
+  return n;
+}
 
 }  // namespace
 
 // desc | parts' O | parts' (max, sum), for the largest launch
 size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
   if (T == 0) return 0;
-  const size_t G = nq / nkv, cols = attn_rows((int)G) * G;
+  const size_t G = nq / nkv, cols = attn_rows((int)G, 2) * G;
   return kPaMaxCtas * (sizeof(int4) + 2 * cols * (hd * sizeof(float) + sizeof(float2)));
 }
 
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
+  // Two column tiles where one row needs them, or where a request has the rows
+  // to fill them on average and there are three such groups for two SMs: the
+  // keys are read and turned into operands half as often. One tile -> two:
+  // 256 rows in chunks of 64, 24/4 heads of 128, bf16: 93.9 -> 79.0 us; 170 rows
+  // 50.9 -> 44.6; 512 rows in chunks of 4: 290 -> 221, of 2: 301 -> 220. Not so
+  // for 8/8 heads of 64, e4m3: 512 rows in chunks of 8 (half a tile): 45 -> 62,
+  // of 16: 43 -> 38; 320 rows (160 groups): 19.4 -> 20.6.
+  const int wide = attn_rows(G, 2);
+  const bool many =
+      a.req && wide > attn_rows(G, 1) && a.T / wide >= a.n_req && (long long)a.T * a.nq >= 24 * 148;
+  const int nt = G > 8 || many ? 2 : 1;
   int id;
   size_t smem;
-  const AttnKernel k = attn_kernel(a.kv.hd, e4m3, G, &id, &smem);
+  const AttnKernel k = attn_kernel(a.kv.hd, e4m3, nt, &id, &smem);
   const int full = attn_ctas(k, id, smem);
   if (full < 1) return SLX_ERR_CUDA;
   // no more CTAs than steps (a unit per warp) the rows could fill
@@ -1463,7 +1479,7 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
     const long long steps = (segs * row_units + kPaWarps - 1) / kPaWarps;
     if (steps < full) grid = (int)steps;
   }
-  const int rpb = a.req ? attn_rows(G) : 1, cols = rpb * G;
+  const int rpb = a.req ? attn_rows(G, nt) : 1, cols = rpb * G;
   PaWork ws;
   uint8_t* p = reinterpret_cast<uint8_t*>(a.ws);
   ws.desc = reinterpret_cast<int4*>(p);

@@ -166,6 +166,46 @@ def test_attention_long_prompt_rows(dtype):
     check_attention(queries(51, 4, 64), host, dev, req, pos)
 
 
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("nq,nkv,hd,T", [
+    (8, 8, 64, 460), (24, 4, 128, 160), (9, 3, 64, 410), (16, 2, 128, 240),
+    (12, 4, 128, 300), (32, 2, 64, 140)])
+def test_attention_many_prompt_rows(nq, nkv, hd, T, dtype):
+    """Chunks long enough for the wider tile: ragged, some of a row, padding
+    and idle rows between them, values of later tokens that are not finite."""
+    g = np.random.default_rng(T)
+    lens = [400, 37, 290, 64]
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=T)
+    pages = host[0].float()
+    for i, n in ((0, 190), (2, 120)):
+        pages[int(host[2][i, n // 16]), 1, :, n % 16] = \
+            float("inf") if dtype == BF and i else float("nan")
+    pages = pages.to(dtype)
+    req, pos = [], []
+    while len(req) < T:
+        i = int(g.integers(-1, 4))
+        n = min(T - len(req), int(g.choice([1, 3, 16, 29, 70])))
+        if i < 0:
+            req += [-1] * min(n, 3)
+            pos += [-1] * min(n, 3)
+            continue
+        n = min(n, lens[i])
+        at = int(g.integers(0, lens[i] - n + 1))
+        req += [i] * n
+        pos += range(at, at + n)
+    last = {0: 190, 1: 37, 2: 120, 3: 64}
+    clean = [r for r in range(T) if req[r] < 0 or pos[r] < last[req[r]]]
+    rest = [r for r in range(T) if req[r] >= 0 and pos[r] >= last[req[r]]]
+    assert len(rest) > 0
+    q = queries(T, nq, hd)
+    out, st = run_attention(q, (pages.cuda(), dev[1], dev[2]), req, pos)
+    assert st == 0 and not torch.isfinite(out[rest]).any()
+    want, bound = P.attention(q[clean], pages, host[1], host[2],
+                              [req[r] for r in clean],
+                              [pos[r] for r in clean], 16, hd ** -0.5)
+    assert ((out[clean].double() - want).abs() <= bound).all()
+
+
 def test_attention_strided_queries():
     """q as the head part of wider rows, and a row stride beyond them."""
     lens = [40, 7, 90]
