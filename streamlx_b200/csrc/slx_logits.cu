@@ -51,6 +51,10 @@ template <>
 struct Raw8<uint16_t> {
   uint32_t w[4];
   SLX_DEV float get(int j) const { return j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]); }
+  SLX_DEV uint16_t bits(int j) const {
+    const uint32_t lo = j & 2 ? w[1] : w[0], hi = j & 2 ? w[3] : w[2], x = j & 4 ? hi : lo;
+    return (uint16_t)(j & 1 ? x >> 16 : x);
+  }
   SLX_DEV void put(int j, uint16_t b) {
     w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | ((uint32_t)b << 16) : (w[j / 2] & 0xffff0000u) | b;
   }
@@ -84,13 +88,19 @@ struct Raw8<uint16_t> {
   }
   SLX_DEV void load1(int j, const uint16_t* p) { put(j, *p); }
   SLX_DEV void store1(int j, uint16_t* p) const {
-    *p = (uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
+    *p = bits(j);
   }
 };
 template <>
 struct Raw8<float> {
   float f[8];
   SLX_DEV float get(int j) const { return f[j]; }
+  SLX_DEV float bits(int j) const {
+    float x = f[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) x = i == j ? f[i] : x;
+    return x;
+  }
   SLX_DEV void mask(uint32_t keep) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -135,20 +145,28 @@ SLX_DEV void warp_best(uint64_t& key, int& id) {
 // A cluster of 8 CTAs per row; runs of 32 vectors of eight ids (a warp's
 // load) go round the CTAs, because the ids that rules touch crowd at the
 // vocabulary's start and the cluster waits for its slowest CTA.  Every thread
-// requests its history entries and mask bits, then the logits that some bit
-// allows (16-byte loads, all in flight together), and while they come the CTA
-// builds its ids' words: zero, biases, history.  The vectors are then copied
-// (masked ids -inf) and the touched ids listed; a second pass computes the
-// list with whole warps, in fp64, so picks between neighbouring values do not
-// depend on the rounding of an intermediate.  Bound by HBM for a batch (each
-// logit read and written once, masked ones not read) and by the words' shared
-// memory, which holds the CTAs per SM at two; for one row by the chain
-// history -> words -> copy -> list -> cluster reduction.
+// requests its history entries, the logits (16-byte loads, all in flight
+// together, before the mask's words are there) and the mask's words, and while
+// they come the CTA builds its ids' words: zero, history (each pass over it
+// two loads ahead), biases.  The vectors are then copied (masked ids -inf) and
+// the touched ids listed with their values; a second pass computes the list
+// with whole warps, in fp64, so picks between neighbouring values do not
+// depend on the rounding of an intermediate.  Bound for a batch by those
+// phases, one behind the other in the two CTAs that an SM holds (the words'
+// shared memory, 64 registers a thread): 38 % of the issue slots, DRAM at a
+// quarter; 128 rows of 151936 in bf16 with 8000 past tokens each, cold: 63 us,
+// 70 before the logits were asked for ahead of the mask and the list held its
+// values.  A bitmap of touched ids with counts for those alone (a quarter of
+// the shared memory, four CTAs of 256 threads) goes over the history twice:
+// 90 us; the history split over the cluster, counted by atomics into the other
+// CTAs' shared memory: 80 us.  For one row by the chain history -> words ->
+// copy -> list -> cluster reduction.
 template <typename T>
 __global__ void __cluster_dims__(kLogitCluster, 1, 1)
     __launch_bounds__(kLogitThreads, 2) k_logits(const LogitArgs a) {
   extern __shared__ __align__(16) uint32_t s_word[];
   __shared__ uint16_t s_list[kLogitList];
+  __shared__ T s_val[kLogitList];
   __shared__ int s_n;
   __shared__ uint64_t s_key[kLogitThreads / 32], c_key[kLogitCluster];
   __shared__ int s_id[kLogitThreads / 32], c_id[kLogitCluster];
@@ -186,6 +204,7 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
   int h0 = 0;
   constexpr int kAhead = 2;
   int4 ahead[kAhead];
+  float rep = 1.f, freq = 0.f, pres = 0.f;
   if (R.history) {
     h0 = (int)((16 - (reinterpret_cast<uintptr_t>(hist) & 15)) / 4 % 4);
 #pragma unroll
@@ -195,6 +214,9 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
     }
     n_hist = R.n_history[row];
     n_prompt = R.n_prompt ? R.n_prompt[row] : 0;
+    if (R.repetition) rep = R.repetition[row];
+    if (R.frequency) freq = R.frequency[row];
+    if (R.presence) pres = R.presence[row];
   }
   if (R.bias_ids) {
     bias0 = R.bias_start[row];
@@ -204,15 +226,29 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
   for (int q0 = 0; q0 < q_end; q0 += KV * kLogitThreads) {
     const int kb = vec_at(q0 + tid), idb = 8 * kb - lead;
     auto whole = [&](int id) { return id >= 0 && id <= a.V - 8; };
-    // allowed bits of each vector (ids outside the row are not allowed)
-    uint32_t ok[KV];
     Raw8<T> raw[KV];
+    uint32_t ok[KV];  // allowed bits of each vector (ids outside the row are not)
 #pragma unroll
     for (int v = 0; v < KV; ++v) {
       const int id = idb + v * hop * 8;
       ok[v] = kb + v * hop < n_vec ? 0xffu : 0u;
-      if (mask && ok[v]) {
+      if (!ok[v]) continue;
+      if (whole(id)) {
+        raw[v].load(x_row + id);
+      } else {
+        if (id < 0) ok[v] &= 0xffu << -id;
+        if (id > a.V - 8) ok[v] &= 0xffu >> (id + 8 - a.V);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (ok[v] >> j & 1) raw[v].load1(j, x_row + id + j);
+      }
+    }
+    if (mask) {
+#pragma unroll
+      for (int v = 0; v < KV; ++v) {
+        if (!ok[v]) continue;
         // (hop * 8 is a multiple of 32: the same shift for every vector)
+        const int id = idb + v * hop * 8;
         const int i0 = max(id, 0) >> 5, i1 = min(id + 7, a.V - 1) >> 5;
         const uint32_t w0 = mask[i0];
         if (lead == 0)
@@ -220,22 +256,13 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
         else
           ok[v] &= id < 0 ? w0 << -id : __funnelshift_r(w0, mask[i1], idb & 31);
       }
-      if (ok[v] && !whole(id)) {
-        if (id < 0) ok[v] &= 0xffu << -id;
-        if (id > a.V - 8) ok[v] &= 0xffu >> (id + 8 - a.V);
-      }
     }
-#pragma unroll
-    for (int v = 0; v < KV; ++v) {
-      const int id = idb + v * hop * 8;
-      if (!ok[v]) continue;
-      if (whole(id)) {
-        raw[v].load(x_row + id);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (ok[v] >> j & 1) raw[v].load1(j, x_row + id + j);
-      }
+    if (R.history || R.bias_ids) {
+      const int n_id = min(q_end - q0, KV * kLogitThreads) * 8;
+      if (q0 > 0) __syncthreads();
+      for (int i = tid; i < n_id / 4; i += kLogitThreads)
+        reinterpret_cast<uint4*>(s_word)[i] = make_uint4(0, 0, 0, 0);
+      if (tid == 0) s_n = 0;
     }
     if (q0 == 0) {
       bool bad = n_hist < 0 || n_hist > R.history_stride || n_prompt < 0 || n_prompt > n_hist;
@@ -262,19 +289,8 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
         return (unsigned)id < (unsigned)a.V && run % kLogitCluster == (unsigned)rank
                    ? (run / kLogitCluster << 8 | (e & 255u)) - base : 0xffffffffu;
       };
+      const int b_first = bias0 + tid < bias1 ? R.bias_ids[bias0 + tid] : -1;
       __syncthreads();
-      for (int i = tid; i < n_id / 4; i += kLogitThreads)
-        reinterpret_cast<uint4*>(s_word)[i] = make_uint4(0, 0, 0, 0);
-      if (tid == 0) s_n = 0;
-      __syncthreads();
-      if (bias1 > bias0) {
-        for (int e = bias0 + tid; e < bias1; e += kLogitThreads) {
-          const unsigned at = place(R.bias_ids[e]);
-          if (at < (unsigned)n_id)
-            atomicMax(s_word + at, (uint32_t)(e - bias0 + 1) << kBiasShift);
-        }
-        __syncthreads();
-      }
       auto note = [&](int id, int e) {
         const unsigned at = place(id);
         if (at >= (unsigned)n_id) return;
@@ -290,16 +306,45 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
         note(q.z, e + 2);
         note(q.w, e + 3);
       };
+      if (q0 > 0) {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int e = h0 + 4 * (tid + i * kLogitThreads);
-        if (e < n_hist - 3) note4(ahead[i], e);
+        for (int i = 0; i < kAhead; ++i) {
+          const int e = h0 + 4 * (tid + i * kLogitThreads);
+          if (e < n_hist - 3) ahead[i] = *reinterpret_cast<const int4*>(hist + e);
+        }
       }
 #pragma unroll 1
-      for (int e = h0 + 4 * (tid + kAhead * kLogitThreads); e < n_hist - 3; e += 4 * kLogitThreads)
-        note4(*reinterpret_cast<const int4*>(hist + e), e);
+      for (int e = h0 + 4 * tid;; e += 4 * kAhead * kLogitThreads) {
+        int4 now[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          now[i] = ahead[i];
+          const int en = e + 4 * (kAhead + i) * kLogitThreads;
+          if (en < n_hist - 3) ahead[i] = *reinterpret_cast<const int4*>(hist + en);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+          if (e + 4 * i * kLogitThreads < n_hist - 3) note4(now[i], e + 4 * i * kLogitThreads);
+        if (e + 4 * kAhead * kLogitThreads >= n_hist - 3) break;
+      }
       const int h1 = h0 + (n_hist - h0) / 4 * 4 + tid;
       if (h1 < n_hist) note(hist[h1], h1);
+      // the row's last entry of an id stands
+      auto bias = [&](int id, int e) {
+        const unsigned at = place(id);
+        if (at >= (unsigned)n_id) return;
+        const uint32_t field = (uint32_t)(e - bias0 + 1) << kBiasShift;
+        uint32_t old = reinterpret_cast<volatile uint32_t*>(s_word)[at];
+        while ((old & ~kPrompt) >> kBiasShift < (uint32_t)(e - bias0 + 1)) {
+          const uint32_t w = (old & (kPrompt | kCountMask)) | field;
+          const uint32_t was = atomicCAS(s_word + at, old, w);
+          if (was == old) break;
+          old = was;
+        }
+      };
+      bias(b_first, bias0 + tid);
+      for (int e = bias0 + tid + kLogitThreads; e < bias1; e += kLogitThreads)
+        bias(R.bias_ids[e], e);
       __syncthreads();
     }
     float pass = -INFINITY;  // best of this pass's ids that no rule touches,
@@ -318,8 +363,13 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
       }
       if (uint32_t list = touched & ok[v]) {
         int at = atomicAdd(&s_n, __popc(list));
-        for (; list; list &= list - 1, ++at)
-          if (at < kLogitList) s_list[at] = (uint16_t)(q * 8 + __ffs(list) - 1);
+        for (; list; list &= list - 1, ++at) {
+          const int j = __ffs(list) - 1;
+          if (at < kLogitList) {
+            s_list[at] = (uint16_t)(q * 8 + j);
+            s_val[at] = raw[v].bits(j);
+          }
+        }
       }
       if (ok[v]) first = min(first, id + __ffs(ok[v]) - 1);
       if (ok[v] != 0xffu) raw[v].mask(ok[v]);
@@ -363,9 +413,6 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
     if (words) {
       const int n_id = min(q_end - q0, KV * kLogitThreads) * 8;
       __syncthreads();  // the copied vectors are written (out may be logits)
-      const double rep = R.repetition ? (double)R.repetition[row] : 1.0;
-      const double freq = R.frequency ? (double)R.frequency[row] : 0.0;
-      const double pres = R.presence ? (double)R.presence[row] : 0.0;
       const bool listed = s_n <= kLogitList;
       const int n = listed ? s_n : n_id;
 #pragma unroll 1
@@ -373,11 +420,11 @@ __global__ void __cluster_dims__(kLogitCluster, 1, 1)
         const int i = listed ? s_list[t] : t;
         const uint32_t w = s_word[i];
         const int id = 8 * vec_at(q0 + (i >> 3)) - lead + (i & 7);
-        if (!w || (mask && !(mask[id >> 5] >> (id & 31) & 1u))) continue;
-        double x = to_f32(x_row[id]);
+        if (!listed && (!w || (mask && !(mask[id >> 5] >> (id & 31) & 1u)))) continue;
+        double x = to_f32(listed ? s_val[t] : x_row[id]);
         const uint32_t c = w & kCountMask;
-        if (c || (w & kPrompt)) x = x > 0.0 ? x / rep : x * rep;
-        if (c) x = __dsub_rn(__dsub_rn(x, __dmul_rn(freq, (double)c)), pres);
+        if (c || (w & kPrompt)) x = x > 0.0 ? x / (double)rep : x * (double)rep;
+        if (c) x = __dsub_rn(__dsub_rn(x, __dmul_rn((double)freq, (double)c)), (double)pres);
         const int e = (int)((w & ~kPrompt) >> kBiasShift);
         if (e) x = __dadd_rn(x, (double)R.bias_values[bias0 + e - 1]);
         best.take(x, id);
