@@ -22,6 +22,10 @@ from . import _lib as L
 from . import ops
 
 
+MAX_BIAS = 8191         # biased ids of a request
+MAX_HISTORY = 262143    # tokens of a request with penalties
+
+
 @dataclass
 class LogitRules:
     """What one request's logits go through before the pick."""
@@ -32,6 +36,26 @@ class LogitRules:
     # grammar: called with the request's output ids, returns uint32 words
     # (bit i of word w allows id 32 w + i) or None for "anything"
     mask: object = None
+
+    @property
+    def penalises(self) -> bool:
+        return bool(self.repetition != 1 or self.frequency or self.presence)
+
+    def check(self, vocab: int, tokens: int) -> None:
+        """Raise ValueError unless a request of ``tokens`` tokens can have
+        these rules."""
+        if not self.repetition > 0:
+            raise ValueError(f"repetition {self.repetition}: must be positive")
+        if self.frequency != self.frequency or self.presence != self.presence:
+            raise ValueError("frequency and presence must be numbers")
+        if self.penalises and tokens > MAX_HISTORY:
+            raise ValueError(f"{tokens} tokens: penalties reach "
+                             f"{MAX_HISTORY} at most")
+        if len(self.bias) > MAX_BIAS:
+            raise ValueError(f"{len(self.bias)} biases: {MAX_BIAS} at most")
+        for i, v in self.bias.items():
+            if not 0 <= i < vocab or v != v:
+                raise ValueError(f"bias {v} of id {i} (vocabulary {vocab})")
 
 
 class PagedKVCache:
@@ -86,7 +110,12 @@ class BatchDecoder:
     is admitted when the pages of its prompt and ``max_new`` tokens are free,
     so a running one never runs out.  The pools' bookkeeping is the eager
     path's (one host sync on the routed ids per layer); single-request decode
-    through the step graph stays ``SynthDecoder.step``."""
+    through the step graph stays ``SynthDecoder.step``, and so does its
+    temporal-reuse routing override (``repeat_p``), which does not apply here.
+
+    A mask that raises, or whose words do not fit, leaves the requests as they
+    were.  When a step fails later than that (a device error, an interrupt)
+    its requests are lost: further steps raise, build a new decoder."""
 
     def __init__(self, model, max_requests: int = 8, max_tokens: int = 1024,
                  n_pages: int | None = None, page_size: int = 64,
@@ -101,6 +130,12 @@ class BatchDecoder:
         if max_requests < 1 or max_tokens < 1 or prompt_chunk < 1:
             raise ValueError("max_requests, max_tokens and prompt_chunk must "
                              "be positive")
+        if page_size not in ops.PAGE_SIZES:
+            raise ValueError(f"page_size {page_size}: one of {ops.PAGE_SIZES}")
+        if cfg.head_dim not in (64, 128) or cfg.heads > 16 * cfg.kv_heads:
+            raise ValueError(f"batched decode needs heads of 64 or 128 and at "
+                             f"most 16 of them a kv head, not {cfg.head_dim} "
+                             f"and {cfg.heads}/{cfg.kv_heads}")
         self.model, self.cfg, self.device = model, cfg, model.device
         self.max_tokens, self.chunk = max_tokens, prompt_chunk
         if n_pages is None:
@@ -117,6 +152,7 @@ class BatchDecoder:
         self._queue: deque = deque()
         self._next_id = 0
         self._reserved = 0              # pages promised to running requests
+        self._failed = False            # a step did not come to its end
         i32 = dict(dtype=torch.int32, device=self.device)
         self.status = torch.zeros(1, **i32)
         self.history = torch.zeros(max_requests, max_tokens, **i32)
@@ -149,6 +185,8 @@ class BatchDecoder:
             raise ValueError(f"{total} tokens do not fit the cache "
                              f"({self.max_tokens} a request, "
                              f"{self.cache.n_pages} pages)")
+        if rules is not None:
+            rules.check(self.cfg.vocab, total)
         r = _Request(self._next_id, prompt, max_new, rules, eos)
         self._next_id += 1
         self._queue.append(r)
@@ -183,27 +221,60 @@ class BatchDecoder:
         """One step of every running request: its next prompt chunk, or its
         last token.  Returns {request id: picked token} of the requests past
         their prompts; a request whose mask allows nothing ends with -1."""
+        if self._failed:
+            raise RuntimeError("an earlier step of this decoder failed and "
+                               "its requests are lost: build a new one")
         with torch.cuda.device(self.device):
-            return self._step()
+            self._admit()
+            counts = self._rows_of_slots()
+            masks = self._masks(counts)
+            self._failed = True
+            got = self._step(counts, masks)
+            self._failed = False
+        return got
 
-    def _step(self) -> dict[int, int]:
-        self.model.flush()
-        self._admit()
-        n_new, ids, from_last, picking = [], [], [], []
+    def _rows_of_slots(self) -> list[int]:
+        """Rows of each slot's request in the next step (-1: its pages go
+        back)."""
+        n = []
         for s, r in enumerate(self.slots):
             if r is None:
-                n_new.append(-1 if s in self._gone else 0)
+                n.append(-1 if s in self._gone else 0)
+            else:
+                n.append(min(max(len(r.prompt) - r.fed, 1), self.chunk))
+        return n
+
+    def _masks(self, counts) -> dict:
+        """{slot: mask words} of the requests that the step picks for."""
+        words, out = (self.cfg.vocab + 31) // 32, {}
+        for s, (r, n) in enumerate(zip(self.slots, counts)):
+            if r is None or r.fed + n < len(r.prompt):
                 continue
-            left = len(r.prompt) - r.fed
-            n = min(left, self.chunk) if left > 0 else 1
-            n_new.append(n)
-            if left > 0:
+            if r.rules is None or r.rules.mask is None:
+                continue
+            w = r.rules.mask(list(r.out))
+            if w is not None:
+                w = np.asarray(w, dtype=np.uint32)
+                if w.ndim != 1 or len(w) < words:
+                    raise ValueError(f"request {r.rid}: mask of shape "
+                                     f"{w.shape}, {words} words wanted")
+                out[s] = w[:words]
+        return out
+
+    def _step(self, n_new, masks) -> dict[int, int]:
+        self.model.flush()
+        ids, from_last, picking = [], [], []
+        for s, r in enumerate(self.slots):
+            if r is None:
+                continue
+            n = n_new[s]
+            if r.fed < len(r.prompt):
                 ids += r.prompt[r.fed:r.fed + n]
             else:
                 from_last.append((len(ids), s))
                 ids.append(0)
             r.fed += n
-            if left <= n:
+            if r.fed >= len(r.prompt):
                 picking.append((s, len(ids) - 1))   # slot, its last row
         dev = self.device
         rows = len(ids)
@@ -228,7 +299,7 @@ class BatchDecoder:
                                   dtype=torch.bfloat16, device=dev)
         L.qlinear(self.model.w_lm, self.cfg.vocab, self.cfg.hidden,
                   self.cfg.trunk_bits, x, self.logits, self.status)
-        return self._pick(slots)
+        return self._pick(slots, masks)
 
     def _forward(self, tok, plan) -> torch.Tensor:
         """Hidden rows (after the final norm) of the step's tokens."""
@@ -265,7 +336,7 @@ class BatchDecoder:
         L.add_rmsnorm(h, delta, m.norm, cfg.rms_eps, x)
         return x
 
-    def _pick(self, slots) -> dict[int, int]:
+    def _pick(self, slots, masks) -> dict[int, int]:
         """Rules, greedy pick and the requests' state after it."""
         dev, V = self.device, self.cfg.vocab
         reqs = [self.slots[s] for s in slots]
@@ -273,7 +344,7 @@ class BatchDecoder:
         at = torch.tensor(slots, device=dev)
         n_hist = [len(r.prompt) + len(r.out) for r in reqs]
         kw = {}
-        if any(u.repetition != 1 or u.frequency or u.presence for u in rules):
+        if any(u.penalises for u in rules):
             kw = {name: torch.tensor([getattr(u, name) for u in rules],
                                      dtype=torch.float32).to(dev)
                   for name in ("repetition", "frequency", "presence")}
@@ -288,13 +359,12 @@ class BatchDecoder:
             kw["bias"] = (torch.tensor(ids, dtype=torch.int32).to(dev),
                           torch.tensor(vals, dtype=torch.float32).to(dev),
                           torch.from_numpy(start).to(dev))
-        if any(u.mask is not None for u in rules):
-            words = (V + 31) // 32
-            m = np.full((len(reqs), words), 0xFFFFFFFF, dtype=np.uint32)
-            for i, (r, u) in enumerate(zip(reqs, rules)):
-                w = u.mask(list(r.out)) if u.mask is not None else None
-                if w is not None:
-                    m[i] = np.asarray(w, dtype=np.uint32)[:words]
+        if masks:
+            m = np.full((len(reqs), (V + 31) // 32), 0xFFFFFFFF,
+                        dtype=np.uint32)
+            for i, s in enumerate(slots):
+                if s in masks:
+                    m[i] = masks[s]
             kw["mask"] = torch.from_numpy(m.view(np.int32)).to(dev)
         pick = ops.process_logits(self.logits, status=self.status, **kw)
         self.last[at] = pick
@@ -323,7 +393,11 @@ class BatchDecoder:
     def generate(self, prompts, max_new: int, rules=None,
                  eos: int | None = None) -> list[list[int]]:
         """Every prompt to its end; ``rules``: one LogitRules, or one per
-        prompt.  A mask that allows nothing ends a request without a token."""
+        prompt.  A mask that allows nothing ends a request without a token.
+        Not while submitted requests run: their tokens come from ``step``."""
+        if self.busy:
+            raise RuntimeError("generate: submitted requests are running, "
+                               "their tokens come from step")
         if not isinstance(rules, (list, tuple)):
             rules = [rules] * len(prompts)
         if len(rules) != len(prompts):
@@ -332,7 +406,7 @@ class BatchDecoder:
         out: dict = {i: [] for i in ids}
         while self.busy:
             for rid, t in self.step().items():
-                if t >= 0 and rid in out:
+                if t >= 0:
                     out[rid].append(t)
         self.release()
         return [out[i] for i in ids]

@@ -186,3 +186,59 @@ def test_refusals(tiny):
         dec.generate([[1], [2]], 2, rules=[None])
     assert dec.generate([], 3) == []
     reader.close()
+
+
+def test_rules_are_checked(tiny):
+    """Rules that would end a step of everyone's are refused at once."""
+    cfg, model, reader = load(tiny["tiny_dec"])
+    dec = BatchDecoder(model, max_requests=2, max_tokens=20, page_size=16)
+    nan = float("nan")
+    for bad in (LogitRules(repetition=0.0), LogitRules(repetition=nan),
+                LogitRules(frequency=nan), LogitRules(presence=nan),
+                LogitRules(bias={cfg.vocab: 1.0}), LogitRules(bias={-1: 1.0}),
+                LogitRules(bias={0: nan}),
+                LogitRules(bias=dict.fromkeys(range(8192), 1.0))):
+        with pytest.raises(ValueError):
+            dec.submit([1, 2], 3, bad)
+    with pytest.raises(ValueError):
+        LogitRules(presence=1.0).check(cfg.vocab, 262144)
+    LogitRules(bias={0: float("-inf")}).check(cfg.vocab, 262144)
+    assert not dec.busy
+    reader.close()
+
+
+def test_failed_masks_and_steps(tiny):
+    """A mask that raises or does not fit changes nothing; a step that fails
+    later ends the decoder."""
+    cfg, model, reader = load(tiny["tiny_dec"])
+    prompt = np.random.default_rng(9).integers(0, cfg.vocab, 9).tolist()
+    want = model.generate_batch([prompt], 5)[0]
+    dec = BatchDecoder(model, max_requests=2, max_tokens=20, page_size=16,
+                       prompt_chunk=4)
+    bad = [ValueError("no state"), np.zeros(1, np.uint32)]
+
+    def mask(out):
+        if len(out) == 2 and bad:
+            w = bad.pop()
+            if isinstance(w, Exception):
+                raise w
+            return w
+        return None
+
+    dec.submit(prompt, 5, LogitRules(mask=mask))
+    got, failures = [], 0
+    while dec.busy:
+        try:
+            got += dec.step().values()
+        except ValueError:
+            failures += 1
+    assert failures == 2 and got == want
+    with pytest.raises(RuntimeError):
+        dec.submit(prompt, 2)
+        dec.generate([prompt], 2)
+    dec._forward = None             # a step that fails on its way
+    with pytest.raises(TypeError):
+        dec.step()
+    with pytest.raises(RuntimeError, match="lost"):
+        dec.step()
+    reader.close()
