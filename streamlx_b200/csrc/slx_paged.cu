@@ -6,7 +6,9 @@
 #include <cooperative_groups.h>
 #include <cuda_fp8.h>
 
-#include "slx_kernels.cuh"
+#include <algorithm>
+
+#include "slx_paged.cuh"
 
 namespace slx {
 
@@ -218,11 +220,6 @@ int launch_paged_plan(const PlanArgs& a, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------- append --
-
-SLX_DEV uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 // four values to e4m3, to nearest, saturating at 448
 SLX_DEV uint32_t f32x4_to_e4m3(const float (&x)[4]) {
@@ -444,12 +441,6 @@ struct PaWork {       // workspace of one call
   float2* ml;         // [2 CTAs][cols] max (log2), sum; sum -1: no such row
 };
 
-SLX_DEV float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 SLX_DEV void ld_stream(const uint8_t* p, uint32_t* v) {
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
@@ -474,30 +465,6 @@ SLX_DEV uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
-}
-
-// four e4m3 bytes -> two fp16 pairs (exact; NaN stays NaN)
-SLX_DEV void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{.reg .b16 t, u; mov.b32 {t, u}, %2; cvt.rn.f16x2.e4m3x2 %0, t; "
-      "cvt.rn.f16x2.e4m3x2 %1, u;}"
-      : "=r"(lo), "=r"(hi) : "r"(w));
-}
-
-// Row t's request and the keys it attends: pos + 1, 0 for an idle row or one
-// out of range.  (Both are read at once: rows are read in batches.)
-struct RowKeys {
-  int req, pos, keys;
-};
-SLX_DEV RowKeys row_keys(const PagedAttnArgs& a, int t) {
-  RowKeys r = {0, -1, 0};
-  if (t < a.T) {
-    r.pos = a.pos[t];
-    r.req = a.req ? a.req[t] : t;
-  }
-  const bool ok = (unsigned)r.req < (unsigned)a.n_req &&
-                  (unsigned)r.pos >> a.kv.page_shift < (unsigned)a.max_pages && r.pos >= 0;
-  r.keys = ok ? r.pos + 1 : 0;
-  return r;
 }
 
 // Rows are taken in aligned blocks of `rpb` (a power of two up to 16: what fits
@@ -1449,11 +1416,13 @@ int attn_rows(int G, int nt) {
 size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
   if (T == 0) return 0;
   const size_t G = nq / nkv, cols = attn_rows((int)G, 2) * G;
-  return kPaMaxCtas * (sizeof(int4) + 2 * cols * (hd * sizeof(float) + sizeof(float2)));
+  const size_t n = kPaMaxCtas * (sizeof(int4) + 2 * cols * (hd * sizeof(float) + sizeof(float2)));
+  return std::max(n, paged_tile_workspace_bytes(nq, nkv, hd));
 }
 
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
+  if (a.req && a.T / (128 / G) >= a.n_req) return launch_paged_tile(a, e4m3, s);
   // Two column tiles where one row needs them, or where a request has the rows
   // to fill them on average and there are three such groups for two SMs: the
   // keys are read and turned into operands half as often. One tile -> two:

@@ -66,6 +66,7 @@
 // SLX_ERR_DEVICE_TIMEOUT, drains its in-flight copies and MMAs, frees TMEM
 // and returns.
 #include "slx_kernels.cuh"
+#include "slx_tc.cuh"
 #include "slx_tiles.cuh"
 
 // Diagnostics build only (-DSLX_PF_TRACE): %globaltimer stamps of each
@@ -114,91 +115,6 @@ constexpr float kTiny = 7.62939453125e-06f;  // 2^-17: smaller loses bits
 #ifndef SLX_PF_L2_PREFETCH
 #define SLX_PF_L2_PREFETCH 1  // prefetch activation chunks one ring ahead into L2
 #endif
-#ifndef SLX_PF_SLEEP_WAIT
-#define SLX_PF_SLEEP_WAIT 1   // barrier polls with a suspend-time hint
-#endif
-
-// --------------------------------------------------------------- tcgen05 --
-
-SLX_DEV void tc_alloc(uint32_t* dst, int ncols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-               ::"r"(smem_u32(dst)), "r"(ncols) : "memory");
-}
-SLX_DEV void tc_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-SLX_DEV void tc_dealloc(uint32_t taddr, int ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-               ::"r"(taddr), "r"(ncols) : "memory");
-}
-SLX_DEV void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-SLX_DEV void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-// Arrive (once) on `bar` when every MMA this thread issued so far completes.
-SLX_DEV void tc_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-      ::"r"(smem_u32(bar)) : "memory");
-}
-SLX_DEV void tc_mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc,
-                       uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
-}
-SLX_DEV void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]),
-        "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-        "=r"(r[15])
-      : "r"(taddr));
-}
-SLX_DEV void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// Bounded mbarrier wait whose polls let the thread sleep in the hardware
-// (try_wait with a suspend-time hint of 0.2 ms) instead of spinning: the
-// waiting warps then leave their issue slots to the working ones.
-SLX_DEV bool mbar_wait_sleep(uint64_t* bar, uint32_t parity, int32_t* status) {
-  if (!SLX_PF_SLEEP_WAIT) return mbar_wait(bar, parity, status);
-  const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(200000u)
-        : "memory");
-    if (done) return true;
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      set_status(status, SLX_ERR_DEVICE_TIMEOUT);
-      return false;
-    }
-  }
-}
-
-// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row atoms of
-// 1024 bytes stacked along M/N (stride 1024), descriptor version 1.
-SLX_DEV uint64_t sdesc_sw128(uint32_t saddr) {
-  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)1u << 16;              // leading byte offset (unused: swizzled K-major)
-  d |= (uint64_t)(1024u >> 4) << 32;    // stride byte offset
-  d |= (uint64_t)1u << 46;              // version
-  d |= (uint64_t)2u << 61;              // SWIZZLE_128B
-  return d;
-}
-// Instruction descriptor of kind::f16: fp16 A and B (K-major), fp32 D,
-// M = 128, N = n.
-SLX_DEV uint32_t idesc_f16(int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
 
 // ------------------------------------------------------- misc async ops --
 
@@ -211,7 +127,6 @@ SLX_DEV void cp_async4(uint32_t dst, const void* src) {
 SLX_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 SLX_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-SLX_DEV void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Byte offset of fp16 position pos of row n inside a 128-byte-swizzled chunk.
 SLX_DEV int sw_off(int n, int pos) {
   return n * kRowB + ((((pos >> 3) ^ (n & 7))) << 4) + ((pos & 7) << 1);
