@@ -202,6 +202,7 @@ int launch_paged_plan(const PlanArgs& a, cudaStream_t s);
 int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s);
 size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd);
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s);
+int paged_tile_rows(const PagedAttnArgs& a);
 int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s);
 size_t paged_tile_workspace_bytes(int nq, int nkv, int hd);
 int launch_logits(const LogitArgs& a, bool f32, cudaStream_t s);

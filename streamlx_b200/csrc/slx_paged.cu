@@ -1422,17 +1422,23 @@ size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
 
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
-  if (a.req && a.T / (128 / G) >= a.n_req) return launch_paged_tile(a, e4m3, s);
+  // Requests with the rows for 48 columns and more on average, and work for the
+  // device: the kernel for chunks.  This one -> that: 512 rows, 24/4 heads of 128
+  // in bf16, chunks of 8: 215 -> 117 us; 64 rows, 16/2, chunks of 8: 25 -> 17.
+  // Not so for 32 columns (512 rows in chunks of 32, 8/8 heads of 64: 42 -> 53)
+  // or 256 in all (16 rows, 16/2: 16 -> 21).
+  if (a.req && paged_tile_rows(a) * G >= 48 && (long long)a.T * a.nq >= 1024)
+    return launch_paged_tile(a, e4m3, s);
   // Two column tiles where one row needs them, or where a request has the rows
-  // to fill them on average and there are three such groups for two SMs: the
-  // keys are read and turned into operands half as often. One tile -> two:
-  // 256 rows in chunks of 64, 24/4 heads of 128, bf16: 93.9 -> 79.0 us; 170 rows
-  // 50.9 -> 44.6; 512 rows in chunks of 4: 290 -> 221, of 2: 301 -> 220. Not so
-  // for 8/8 heads of 64, e4m3: 512 rows in chunks of 8 (half a tile): 45 -> 62,
-  // of 16: 43 -> 38; 320 rows (160 groups): 19.4 -> 20.6.
-  const int wide = attn_rows(G, 2);
+  // to fill them on average and there is work for the device: the keys are read
+  // and turned into operands half as often.  One tile -> two, 24/4 heads of 128
+  // in bf16: 512 rows in chunks of 4: 290 -> 220 us, of 2: 301 -> 220; 32 rows in
+  // chunks of 4: 33 -> 25, 16 rows: 16.6 -> 19.5.  8/8 heads of 64, e4m3, 512
+  // rows in chunks of 8 (half a tile): 45 -> 62, of 16: 43 -> 38; 64 rows: 15.3
+  // -> 17.1.
+  const int tall = attn_rows(G, 2);
   const bool many =
-      a.req && wide > attn_rows(G, 1) && a.T / wide >= a.n_req && (long long)a.T * a.nq >= 24 * 148;
+      a.req && tall > attn_rows(G, 1) && a.T / tall >= a.n_req && (long long)a.T * a.nq >= 768;
   const int nt = G > 8 || many ? 2 : 1;
   int id;
   size_t smem;

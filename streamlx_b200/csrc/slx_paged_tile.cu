@@ -5,13 +5,39 @@
 
 namespace slx {
 
-// KERNEL COMMENT
+// A CTA takes 128 columns, the (row, q head) pairs of one kv head and of as
+// many rows as fit, over 64 keys at a time:
+//   S [128 x 64] = Q K^T,   O [128 x hd] += P V     (tcgen05.mma, M = 128)
+// with S (twice) and O in TMEM.  A column's lane holds it alone, so maximum and
+// sum need no exchange.  O is scaled only when a column's maximum has grown by
+// 2^8 (P and the sum stay far inside fp32 and fp16 until then); P goes to shared
+// memory as two 16-bit parts, hi + lo, both multiplied: 16 bits or more, as in
+// the kernel for single tokens.  K and V lie in shared memory as their pages
+// have them, rows of 64 dims swizzled over 128 bytes: K-major for S, and for
+// P V with the dims inside (the descriptor's other order), so neither is
+// transposed.  E4m3 keys and values become fp16 on the way (exact), q a power
+// of two times fp16.
+//
+// Warps 0-3: a column each, S -> P, O.  Warps 4, 5 keys and 6, 7 values: global
+// memory to registers a tile ahead, then to the operands; apart, because the
+// fence before the MMAs waits for the loads in flight of its thread.  The first
+// thread of each pair issues its MMAs.  Two CTAs per SM (97 KB each), the keys
+// of a block of rows cut into parts while that leaves the device unfilled; the
+// join adds them in order.
+//
+// Bound by the chain score -> P -> product of a tile (2800 cycles alone on an
+// SM) and, with two CTAs there, by shared memory (operands read by the MMAs 900
+// cycles a tile, P, K and V written 500: 2250 cycles).  4096 rows in chunks of
+// 512 over 4k to 8k keys, 16/2 heads of 128: 475 us in bf16 (425 TFLOP/s
+// without the second part of P), 531 in e4m3, 2214 by the kernel for single
+// tokens.  Values transposed on the way to a K-major operand: 843 us; keys and
+// values by the same threads: 680.
 constexpr int kTileM = 128;       // columns (row, q head): the MMAs' M
 constexpr int kTileKeys = 64;     // keys per tile
 constexpr int kTileThreads = 256;
 constexpr int kTileTmem = 256;    // S twice, O
 constexpr int kTileCtas = 296;    // two per SM
-constexpr int kTileSplits = 16;   // parts of a row at most
+constexpr int kTileSplits = 8;    // parts of a row at most
 constexpr float kTileSlack = 8.f; // a maximum may grow by 2^8 before O is scaled
 
 struct TileWork {
@@ -337,7 +363,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           kr[i * 16 / KK + j] = __ldg(reinterpret_cast<const uint4*>(p + j * KK * RB));
       }
     };
-    auto store = [&](int k0) {
+    // what the operand holds of them: 16-bit elements
+    constexpr int PW = E4M3 ? 2 : 1;
+    uint4 op[E4M3 ? PK : 1][2];
+    auto prepare = [&](int k0) {
       if (k0 + kTileKeys > gr.keys || (held & 15) != 15) {
 #pragma unroll
         for (int j = 0; j < PK; ++j)
@@ -368,25 +397,25 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           atomicMax(&s_odd[gr.r0][1], k0 + j * KK + t / PK);
         }
       }
+      if constexpr (E4M3) {
 #pragma unroll
-      for (int j = 0; j < PK; ++j) {
-        const int key = j * KK + t / PK, piece = t % PK;
-        auto put = [&](int p, uint4 v) {
-          *reinterpret_cast<uint4*>(dst + (p >> 3) * (kTileKeys * 128) + key * 128 +
-                                    (((p & 7) ^ (key & 7)) << 4)) = v;
-        };
-        if constexpr (E4M3) {
-          uint4 x, y;
-          e4m3x4(kr[j].x, x.x, x.y);
-          e4m3x4(kr[j].y, x.z, x.w);
-          e4m3x4(kr[j].z, y.x, y.y);
-          e4m3x4(kr[j].w, y.z, y.w);
-          put(2 * piece, x);
-          put(2 * piece + 1, y);
-        } else {
-          put(piece, kr[j]);
+        for (int j = 0; j < PK; ++j) {
+          e4m3x4(kr[j].x, op[j][0].x, op[j][0].y);
+          e4m3x4(kr[j].y, op[j][0].z, op[j][0].w);
+          e4m3x4(kr[j].z, op[j][1].x, op[j][1].y);
+          e4m3x4(kr[j].w, op[j][1].z, op[j][1].w);
         }
       }
+    };
+    auto store = [&] {
+#pragma unroll
+      for (int j = 0; j < PK; ++j)
+#pragma unroll
+        for (int h = 0; h < PW; ++h) {
+          const int key = j * KK + t / PK, p = t % PK * PW + h;
+          *reinterpret_cast<uint4*>(dst + (p >> 3) * (kTileKeys * 128) + key * 128 +
+                                    (((p & 7) ^ (key & 7)) << 4)) = E4M3 ? op[E4M3 ? j : 0][h] : kr[j];
+        }
     };
     const uint64_t q_desc = sdesc_sw128(smem_u32(sQ)), k_desc = sdesc_sw128(smem_u32(sK));
     const uint64_t p_desc = sdesc_sw128(smem_u32(sP));
@@ -398,11 +427,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       fetch(gr.t0, page_at(gr.t0));
       int page = page_at(gr.t0 + 1);
       for (int tl = gr.t0; tl < gr.t1; ++tl, ++it) {
+        prepare(tl * kTileKeys);
         // K is free when the tile before has its scores, V when it is multiplied
         ok = __all_sync(0xffffffffu, it == 0 || (is_v ? wait(&bar_o, it - 1)
                                                       : wait(&bar_s[(it - 1) & 1], (it - 1) >> 1)));
         if (!ok) break;
-        store(tl * kTileKeys);
+        store();
         fence_proxy_async();
         mbar_arrive(is_v ? &bar_v : &bar_k);
         if (is_v) {
@@ -506,8 +536,16 @@ size_t paged_tile_workspace_bytes(int nq, int nkv, int hd) {
   return kTileCtas * cols * (hd * sizeof(float) + sizeof(float2));
 }
 
+// Rows of a block: as many as fit, or as a request has on average (a block
+// with the rows of several takes them one after the other).
+int paged_tile_rows(const PagedAttnArgs& a) {
+  const int most = kTileM / (a.nq / a.kv.n_kv), each = a.T / a.n_req;
+  return each < most ? (each > 0 ? each : 1) : most;
+}
+
 int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
-  const int nkv = a.kv.n_kv, G = a.nq / nkv, hd = a.kv.hd, rpb = kTileM / G, cols = rpb * G;
+  const int nkv = a.kv.n_kv, G = a.nq / nkv, hd = a.kv.hd, rpb = paged_tile_rows(a);
+  const int cols = rpb * G;
   const long long items = (long long)((a.T + rpb - 1) / rpb) * nkv;
   if (items > 0x7fffffff / kTileSplits) return SLX_ERR_UNSUPPORTED;
   // splits that fill the device, of four tiles and more in the longest request

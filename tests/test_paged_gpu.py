@@ -206,6 +206,174 @@ def test_attention_many_prompt_rows(nq, nkv, hd, T, dtype):
     assert ((out[clean].double() - want).abs() <= bound).all()
 
 
+def chunk_rows(lens, first):
+    """(req, pos): every request's rows from its token first[i] on."""
+    req = [i for i, (n, f) in enumerate(zip(lens, first)) for _ in range(f, n)]
+    return req, [p for n, f in zip(lens, first) for p in range(f, n)]
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("nq,nkv,hd,page,lens,first", [
+    (24, 4, 128, 16, [200, 90, 64], [0, 26, 1]),      # from a request's start
+    (16, 2, 128, 64, [130, 65], [65, 0]),
+    (32, 2, 64, 32, [100, 129], [60, 100]),           # 16 heads a kv head
+    (9, 3, 64, 256, [300, 500], [200, 400]),
+    (13, 1, 128, 16, [150], [30]),                    # columns left over
+    (8, 8, 64, 128, [700, 90], [500, 0]),
+    (1, 1, 128, 16, [1100], [20])])                   # a row a column
+def test_attention_chunks(nq, nkv, hd, page, lens, first, dtype):
+    """Chunks of rows on the wide tiles: heads, pages, tails of every size."""
+    host, dev = dev_cache(lens, nkv, hd, page, dtype, seed=nq)
+    req, pos = chunk_rows(lens, first)
+    assert len(req) * nq >= 1024
+    check_attention(queries(len(req), nq, hd), host, dev, req, pos)
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_chunk_behind_long_prefix(dtype):
+    """Few blocks of rows: their keys split over CTAs, some parts with none
+    that the first rows attend."""
+    lens, first = [9000, 700], [8950, 600]
+    host, dev = dev_cache(lens, 2, 128, 64, dtype, seed=21)
+    req, pos = chunk_rows(lens, first)
+    pos[3], pos[20] = 5, 1000
+    check_attention(queries(len(req), 12, 128), host, dev, req, pos)
+
+
+@pytest.mark.parametrize("scale", [0.0, 40.0, -1.0])
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_chunk_scores(scale, dtype):
+    """Maxima that keep growing (sums are scaled), and hardly grow."""
+    lens, first = [520, 130], [440, 60]
+    pages, sc, table = P.make_cache(lens, 2, 64, 16, dtype, seed=22)
+    x = pages.float()
+    for i, n in enumerate(lens):          # keys grow along the request
+        for p in range(n):
+            x[int(table[i, p // 16]), 0, :, p % 16] *= p / n
+    pages = x.to(dtype)
+    host, dev = (pages, sc, table), (pages.cuda(),
+                                     None if sc is None else sc.cuda(),
+                                     table.cuda())
+    req, pos = chunk_rows(lens, first)
+    check_attention(queries(len(req), 16, 64), host, dev, req, pos, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_chunk_bad_indices(dtype):
+    """Pages, requests and positions out of range in chunks: the status, zeros
+    read or written, the other rows untouched."""
+    lens, first = [200, 150], [100, 60]
+    host, dev = dev_cache(lens, 2, 128, 16, dtype, seed=23)
+    pages, sc, table = dev
+    req, pos = chunk_rows(lens, first)
+    q = queries(len(req), 16, 128)
+    good = check_attention(q, host, dev, req, pos)
+    one = [r for r in range(len(req)) if req[r] == 1]
+    zero = [r for r in range(len(req)) if req[r] == 0]
+    for bad in (-1, pages.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[1, 2] = bad
+        out, st = run_attention(q, (pages, sc, t), req, pos)
+        assert st == L.SLX_ERR_OUT_OF_RANGE
+        assert torch.equal(out[zero], good[zero])
+        clear = host[0].float()
+        clear[int(host[2][1, 2])] = 0
+        want, bound = P.attention(q[one], clear.to(dtype), host[1], host[2],
+                                  [1] * len(one), [pos[r] for r in one], 16,
+                                  128 ** -0.5)
+        assert ((out[one].double() - want).abs() <= bound).all()
+    for r, (i, p) in ((5, (2, 50)), (60, (-1, 50)), (120, (1, 16 * 99)),
+                      (121, (0, 2 ** 31 - 1)), (7, (0, -1))):
+        rq, ps = list(req), list(pos)
+        rq[r], ps[r] = i, p
+        out, st = run_attention(q, dev, rq, ps)
+        rest = [k for k in range(len(req)) if k != r]
+        assert st == (0 if p == -1 else L.SLX_ERR_OUT_OF_RANGE)
+        assert (out[r] == 0).all() and torch.equal(out[rest], good[rest])
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_chunk_infinite_and_nan_keys(dtype):
+    """A NaN key makes the rows that attend it NaN and no other; infinite keys
+    (bf16) follow the formula."""
+    lens, first = [150, 140], [70, 60]
+    host, dev = dev_cache(lens, 1, 64, 16, dtype, seed=24)
+    pages = dev[0]
+    pages[int(host[2][0, 100 // 16]), 0, 0, 100 % 16] = float("nan")
+    q = torch.ones(160, 16, 64, dtype=BF)
+    req, pos = chunk_rows(lens, first)
+    clean = [r for r in range(160) if req[r] == 1 or pos[r] < 100]
+    rest = [r for r in range(160) if r not in clean]
+    if dtype == BF:                        # weight 0 for every row behind it
+        pages[int(host[2][1, 5]), 0, 0, 3] = float("-inf")
+    out, st = run_attention(q, dev, req, pos)
+    assert st == 0 and torch.isnan(out[rest]).all()
+    want, _ = P.attention(q[clean], pages.cpu(), host[1], host[2],
+                          [req[r] for r in clean], [pos[r] for r in clean], 16,
+                          64 ** -0.5)
+    err = (out[clean].double() - want).abs()
+    assert (err <= 2.0 ** -7 * want.abs() + 1e-3).all()
+
+
+def test_attention_chunk_strides_streams_graphs():
+    """Strided queries, the same bits in every call, calls on two streams and
+    in two graphs at once."""
+    lens, first = [1000, 300], [900, 230]
+    host, dev = dev_cache(lens, 2, 128, 16, BF, seed=25)
+    pages, _, table = dev
+    req, pos = (torch.tensor(v, dtype=torch.int32).cuda()
+                for v in chunk_rows(lens, first))
+    T = len(req)
+    wide = torch.randn(T, 20 * 128, generator=torch.Generator().manual_seed(2))
+    q = wide.to(BF).cuda()[:, 256:256 + 16 * 128].unflatten(1, (16, 128))
+    want = ops.paged_attention(q, pages, table, pos, req=req)
+    check_attention(q.cpu(), host, dev, req.tolist(), pos.tolist())
+    ws = ops.paged_workspace(T, 16, 2, 128, "cuda")
+    for _ in range(10):
+        got = ops.paged_attention(q.contiguous(), pages, table, pos, req=req,
+                                  workspace=ws)
+        assert torch.equal(got, want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs, graphs = [], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                outs.append(ops.paged_attention(q, pages, table, pos, req=req))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    for _ in streams:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            a = ops.paged_attention(q, pages, table, pos, req=req)
+            b = ops.paged_attention(a, pages, table, pos, req=req)
+        graphs.append((g, a, b))
+    two = ops.paged_attention(want, pages, table, pos, req=req)
+    torch.cuda.synchronize()
+    for s, (g, _, _) in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, two)
+               for _, a, b in graphs)
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("nq,nkv,hd", [(24, 4, 128), (8, 4, 64), (4, 1, 128)])
+def test_attention_short_chunks(nq, nkv, hd, dtype):
+    """Requests of a few rows each: two column tiles of the kernel for single
+    tokens, more rows than one of its column tiles holds."""
+    g = np.random.default_rng(nq)
+    lens = [int(n) for n in g.integers(20, 300, 60)]
+    each = 4 if nq == 24 else 8
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=26)
+    req, pos = chunk_rows(lens, [n - each for n in lens])
+    req[10], pos[10] = -1, -1
+    out = check_attention(queries(len(req), nq, hd), host, dev, req, pos)
+    assert (out[10] == 0).all()
+
+
 def test_attention_strided_queries():
     """q as the head part of wider rows, and a row stride beyond them."""
     lens = [40, 7, 90]
