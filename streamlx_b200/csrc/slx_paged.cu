@@ -399,7 +399,8 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // with mma.m16n8k16: M is keys / dims, so no row is padding (tcgen05's
 // smallest M of 64 or 128 heads would be).  The columns are the q heads of
 // one row and, where they leave room, of the rows after it that belong to the
-// same request (a prompt's rows share their keys: see lead_keys).
+// same request (a prompt's rows share their keys: see lead_keys; calls whose
+// requests have many rows go to slx_paged_tile.cu).
 //
 // The contraction index of an MMA may be permuted on both sides alike; the
 // fragments are chosen so that each is 16 contiguous bytes of a key.

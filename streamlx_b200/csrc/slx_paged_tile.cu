@@ -413,8 +413,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
         for (int h = 0; h < PW; ++h) {
           const int key = j * KK + t / PK, p = t % PK * PW + h;
-          *reinterpret_cast<uint4*>(dst + (p >> 3) * (kTileKeys * 128) + key * 128 +
-                                    (((p & 7) ^ (key & 7)) << 4)) = E4M3 ? op[E4M3 ? j : 0][h] : kr[j];
+          uint8_t* at = dst + (p >> 3) * (kTileKeys * 128) + key * 128;
+          *reinterpret_cast<uint4*>(at + (((p & 7) ^ (key & 7)) << 4)) =
+              E4M3 ? op[E4M3 ? j : 0][h] : kr[j];
         }
     };
     const uint64_t q_desc = sdesc_sw128(smem_u32(sQ)), k_desc = sdesc_sw128(smem_u32(sK));
