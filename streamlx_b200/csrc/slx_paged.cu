@@ -1425,7 +1425,7 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
   // Requests with the rows for 48 columns and more on average, and work for the
   // device: the kernel for chunks.  This one -> that: 512 rows, 24/4 heads of 128
-  // in bf16, chunks of 8: 215 -> 117 us; 64 rows, 16/2, chunks of 8: 25 -> 17.
+  // in bf16, chunks of 8: 215 -> 109 us; 64 rows, 16/2, chunks of 8: 25 -> 17.
   // Not so for 32 columns (512 rows in chunks of 32, 8/8 heads of 64: 42 -> 53)
   // or 256 in all (16 rows, 16/2: 16 -> 21).
   if (a.req && paged_tile_rows(a) * G >= 48 && (long long)a.T * a.nq >= 1024)

@@ -9,29 +9,28 @@ namespace slx {
 // many rows as fit, over 64 keys at a time:
 //   S [128 x 64] = Q K^T,   O [128 x hd] += P V     (tcgen05.mma, M = 128)
 // with S (twice) and O in TMEM.  A column's lane holds it alone, so maximum and
-// sum need no exchange.  O is scaled only when a column's maximum has grown by
-// 2^8 (P and the sum stay far inside fp32 and fp16 until then); P goes to shared
-// memory as two 16-bit parts, hi + lo, both multiplied: 16 bits or more, as in
-// the kernel for single tokens.  K and V lie in shared memory as their pages
-// have them, rows of 64 dims swizzled over 128 bytes: K-major for S, and for
-// P V with the dims inside (the descriptor's other order), so neither is
-// transposed.  E4m3 keys and values become fp16 on the way (exact), q a power
-// of two times fp16.
+// sum need no exchange.  P takes the place of its scores in TMEM, the second
+// product's first operand, as two 16-bit parts, hi + lo, both multiplied: 16
+// bits or more, as in the kernel for single tokens.  O is scaled only when a
+// column's maximum has grown by 2^8 (P and the sum stay far inside fp32 and fp16
+// until then).  K and V lie in shared memory as their pages have them, rows of
+// 64 dims swizzled over 128 bytes: K-major for S, and for P V with the dims
+// inside (the descriptor's other order), so neither is transposed.  E4m3 keys
+// and values become fp16 on the way (exact), q a power of two times fp16.
 //
 // Warps 0-3: a column each, S -> P, O.  Warps 4, 5 keys and 6, 7 values: global
-// memory to registers a tile ahead, then to the operands; apart, because the
-// fence before the MMAs waits for the loads in flight of its thread.  The first
-// thread of each pair issues its MMAs.  Two CTAs per SM (97 KB each), the keys
-// of a block of rows cut into parts while that leaves the device unfilled; the
-// join adds them in order.
+// memory to registers a tile ahead, then to one of two places; apart, because
+// the fence before the MMAs waits for the loads in flight of its thread.  The
+// first thread of each pair issues its MMAs.  Two CTAs per SM (97 KB each), the
+// keys of a block of rows cut into parts while that leaves the device unfilled;
+// the join adds them in order.
 //
-// Bound by the chain score -> P -> product of a tile (2800 cycles alone on an
-// SM) and, with two CTAs there, by shared memory (operands read by the MMAs 900
-// cycles a tile, P, K and V written 500: 2250 cycles).  4096 rows in chunks of
-// 512 over 4k to 8k keys, 16/2 heads of 128: 475 us in bf16 (425 TFLOP/s
-// without the second part of P), 531 in e4m3, 2214 by the kernel for single
-// tokens.  Values transposed on the way to a K-major operand: 843 us; keys and
-// values by the same threads: 680.
+// Bound by the loads: 2800 cycles a tile alone on an SM, of which a warp of keys
+// takes 1100 to issue its sixteen 512-byte loads, and 2400 a tile with two CTAs;
+// in e4m3 by the conversion.  4096 rows in chunks of 512 over 4k to 8k keys, 16/2
+// heads of 128: 411 us in bf16 (about 470 TFLOP/s without P's second part), 483 in
+// e4m3; 2214 by the kernel for single tokens.  P through shared memory and one
+// place for K and V: 475; values transposed on the way to a K-major operand: 843.
 constexpr int kTileM = 128;       // columns (row, q head): the MMAs' M
 constexpr int kTileKeys = 64;     // keys per tile
 constexpr int kTileThreads = 256;
@@ -63,17 +62,16 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   constexpr int QB = HD / 64 * kTileM * 128;      // Q: chunks of 64 dims, swizzled
   constexpr int KB = HD / 64 * kTileKeys * 128;   // K likewise
   constexpr int VB = KB;                          // V likewise
-  constexpr int PB = kTileM * 128;                // P: 64 keys, high parts, low parts
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_q, bar_k, bar_v, bar_p, bar_o, bar_done;
-  __shared__ __align__(8) uint64_t bar_s[2], bar_free[2];
+  __shared__ __align__(8) uint64_t bar_q, bar_k, bar_v, bar_done;
+  __shared__ __align__(8) uint64_t bar_s[2], bar_p[2], bar_o[2];  // by tile's parity
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ int s_keys[kTileM], s_req[kTileM];
   __shared__ uint32_t s_start[kTileM / 32], s_stop[kTileM / 32];
   __shared__ int s_odd[kTileM][2];  // by group's first row: keys with odd values
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t *sQ = base, *sK = sQ + QB, *sV = sK + KB, *sP = sV + VB;
+  uint8_t *sQ = base, *sK = sQ + QB, *sV = sK + 2 * KB;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nkv = a.kv.n_kv, G = a.nq / nkv, ps = a.kv.page_size, sh = a.kv.page_shift;
   const int split = blockIdx.x % nsplit, item = blockIdx.x / nsplit;
@@ -82,12 +80,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     mbar_init(&bar_q, 128);
     mbar_init(&bar_k, 64);
     mbar_init(&bar_v, 64);
-    mbar_init(&bar_p, 128);
-    mbar_init(&bar_o, 1);
     mbar_init(&bar_done, 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_free[i], 128);
+      mbar_init(&bar_p[i], 128);
+      mbar_init(&bar_o[i], 1);
     }
     s_abort = 0;
     fence_mbar_init();
@@ -214,8 +211,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
           for (int i = 0; i < 4; ++i) tc_ld16(t_lane + b * kTileKeys + 16 * i, r[i]);
           tc_wait_ld();
-          tc_fence_before();
-          mbar_arrive(&bar_free[b]);
           float mx = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -231,10 +226,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           const float f = more ? exp2_fast(m - ms) : 1.f;
           m = top;
           l *= f;
-          // the products with the tile before are done: P is free, O holds
-          ok = it == 0 || __all_sync(0xffffffffu, wait(&bar_o, it - 1));
-          if (!ok) break;
           if (t > gr.t0 && __any_sync(0xffffffffu, more)) {
+            // (the products with the tile before are done)
+            ok = __all_sync(0xffffffffu, wait(&bar_o[1 - b], (it - 1) >> 1));
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < HD / 16; ++i) {
@@ -247,14 +242,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             }
             tc_wait_st();
           }
+          // P takes the scores' place: 32 columns of high parts, 32 of low ones
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t hi[4], lo[4];
+          for (int i = 0; i < 4; ++i) {
+            uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t(&x)[16] = r[i >> 1];
-              const float p0 = exp2_fast(__uint_as_float(x[8 * (i & 1) + 2 * j]) - ms);
-              const float p1 = exp2_fast(__uint_as_float(x[8 * (i & 1) + 2 * j + 1]) - ms);
+            for (int j = 0; j < 8; ++j) {
+              const float p0 = exp2_fast(__uint_as_float(r[i][2 * j]) - ms);
+              const float p1 = exp2_fast(__uint_as_float(r[i][2 * j + 1]) - ms);
               l += p0 + p1;
               if constexpr (!E4M3) {
                 hi[j] = pack_bf16(p0, p1);
@@ -265,15 +260,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 lo[j] = pack_f16x2(p0 - h.x, p1 - h.y);
               }
             }
-            uint8_t* d = sP + tid * 128 + ((i ^ (tid & 7)) << 4);
-            *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(d + PB) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            tc_st8(t_lane + b * kTileKeys + 8 * i, hi);
+            tc_st8(t_lane + b * kTileKeys + kTileKeys / 2 + 8 * i, lo);
           }
-          fence_proxy_async();
+          tc_wait_st();
           tc_fence_before();
-          mbar_arrive(&bar_p);
+          mbar_arrive(&bar_p[b]);
         }
-        ok = ok && __all_sync(0xffffffffu, wait(&bar_o, it - 1));
+        ok = ok && __all_sync(0xffffffffu, wait(&bar_o[(it - 1) & 1], (it - 1) >> 1));
         if (!ok) break;
         tc_fence_after();
       }
@@ -349,7 +343,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     constexpr int PK = RB / 16, KK = 64 / PK;  // 16-byte pieces of a key, keys of a pass
     const bool is_v = warp >= 6;
     const uint8_t* src = a.kv.base + (is_v ? v_off : 0) + t / PK * RB + t % PK * 16;
-    uint8_t* dst = is_v ? sV : sK;
+    uint8_t* dst = is_v ? sV : sK;     // two tiles
     uint4 kr[PK];
     unsigned held = 0;
     auto fetch = [&](int tile, int page) {
@@ -407,19 +401,18 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
       }
     };
-    auto store = [&] {
+    auto store = [&](int b) {
 #pragma unroll
       for (int j = 0; j < PK; ++j)
 #pragma unroll
         for (int h = 0; h < PW; ++h) {
           const int key = j * KK + t / PK, p = t % PK * PW + h;
-          uint8_t* at = dst + (p >> 3) * (kTileKeys * 128) + key * 128;
+          uint8_t* at = dst + b * KB + (p >> 3) * (kTileKeys * 128) + key * 128;
           *reinterpret_cast<uint4*>(at + (((p & 7) ^ (key & 7)) << 4)) =
               E4M3 ? op[E4M3 ? j : 0][h] : kr[j];
         }
     };
     const uint64_t q_desc = sdesc_sw128(smem_u32(sQ)), k_desc = sdesc_sw128(smem_u32(sK));
-    const uint64_t p_desc = sdesc_sw128(smem_u32(sP));
     const uint64_t v_desc = sdesc_sw128_mn(smem_u32(sV), kTileKeys * 128);
     bool ok = true;
     int grp = 0;  // groups with tiles
@@ -429,40 +422,43 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       int page = page_at(gr.t0 + 1);
       for (int tl = gr.t0; tl < gr.t1; ++tl, ++it) {
         prepare(tl * kTileKeys);
-        // K is free when the tile before has its scores, V when it is multiplied
-        ok = __all_sync(0xffffffffu, it == 0 || (is_v ? wait(&bar_o, it - 1)
-                                                      : wait(&bar_s[(it - 1) & 1], (it - 1) >> 1)));
+        // K's place is free when the tile two before has its scores, V's when it
+        // is multiplied
+        const int b = it & 1;
+        ok = __all_sync(0xffffffffu,
+                        it < 2 || wait(is_v ? &bar_o[b] : &bar_s[b], (it >> 1) - 1));
         if (!ok) break;
-        store();
+        store(b);
         fence_proxy_async();
         mbar_arrive(is_v ? &bar_v : &bar_k);
         if (is_v) {
           if (tl + 1 < gr.t1) fetch(tl + 1, page);
           page = page_at(tl + 2);
-          if (t == 0 && wait(&bar_p, it) && wait(&bar_v, it)) {
+          if (t == 0 && wait(&bar_p[b], it >> 1) && wait(&bar_v, it)) {
             tc_fence_after();
             // (descriptors count in 16 bytes)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                tc_mma_ss(tmem + 2 * kTileKeys, p_desc + h * (PB / 16) + 2 * k, v_desc + 128 * k,
+                tc_mma_ts(tmem + 2 * kTileKeys, tmem + b * kTileKeys + h * (kTileKeys / 2) + 8 * k,
+                          v_desc + b * (VB / 16) + 128 * k,
                           (E4M3 ? idesc_f16(HD) : idesc_bf16(HD)) | kIdescBmn,
                           tl > gr.t0 || (h | k) != 0);
-            tc_commit(&bar_o);
+            tc_commit(&bar_o[b]);
           }
         } else {
           if (t == 0 && (tl > gr.t0 || wait(&bar_q, grp)) && wait(&bar_k, it) &&
-              (it < 2 || wait(&bar_free[it & 1], (it >> 1) - 1))) {
+              (it < 2 || wait(&bar_o[b], (it >> 1) - 1))) {
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                tc_mma_ss(tmem + (it & 1) * kTileKeys, q_desc + c * (kTileM * 8) + 2 * k,
-                          k_desc + c * (kTileKeys * 8) + 2 * k,
+                tc_mma_ss(tmem + b * kTileKeys, q_desc + c * (kTileM * 8) + 2 * k,
+                          k_desc + b * (KB / 16) + c * (kTileKeys * 8) + 2 * k,
                           E4M3 ? idesc_f16(kTileKeys) : idesc_bf16(kTileKeys), (c | k) != 0);
-            tc_commit(&bar_s[it & 1]);
+            tc_commit(&bar_s[b]);
           }
           __syncwarp();
           if (tl + 1 < gr.t1) fetch(tl + 1, page);
@@ -560,9 +556,8 @@ int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   using Kernel = void (*)(PagedAttnArgs, TileWork, int, int);
   const Kernel k = hd == 128 ? (e4m3 ? k_paged_tile<128, true> : k_paged_tile<128, false>)
                              : (e4m3 ? k_paged_tile<64, true> : k_paged_tile<64, false>);
-  // Q, K, V^T, P, and what aligns them
-  const size_t smem = (size_t)hd / 64 * (kTileM + kTileKeys) * 128 + (size_t)hd * 128 +
-                      2 * kTileM * 128 + 1024;
+  // Q, two tiles of K and of V, and what aligns them
+  const size_t smem = (size_t)hd / 64 * (kTileM + 4 * kTileKeys) * 128 + 1024;
   static PerDevice configured[4];
   std::atomic<int>& slot = configured[(hd == 128 ? 2 : 0) + e4m3].here();
   if (!slot.load(std::memory_order_relaxed)) {
