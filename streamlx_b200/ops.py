@@ -310,7 +310,8 @@ def paged_plan(n_new: torch.Tensor, lengths: torch.Tensor,
     # rows (request, position, slot), their starts and the state after the
     # step, one allocation
     buf = torch.empty(3 * n_rows + 2 * R + 2, dtype=_I32, device=table.device)
-    req, pos, slot, start, ln, nf = torch.split_with_sizes(
+    # (unsafe: integers, no autograd to track the parts for; 0.6 us less)
+    req, pos, slot, start, ln, nf = torch.unsafe_split_with_sizes(
         buf, (n_rows, n_rows, n_rows, R + 1, R, 1))
     if lengths_out is None:
         lengths_out = ln
@@ -409,7 +410,7 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor,
                          "[n_req, max_pages]")
     n_req, max_pages = table.shape
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     elif (out.dtype is not _BF16 or out.get_device() != idx or
           out.numel() != T * n_q * hd or not out.is_contiguous()):
         raise ValueError("paged_attention: out must be contiguous bfloat16 [T, "
