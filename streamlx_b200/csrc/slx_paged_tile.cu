@@ -25,9 +25,10 @@ namespace slx {
 // keys of a block of rows cut into parts while that leaves the device unfilled;
 // the join adds them in order.
 //
-// Bound by the loads: 2800 cycles a tile alone on an SM, of which a warp of keys
-// takes 1100 to issue its sixteen 512-byte loads, and 2400 a tile with two CTAs;
-// in e4m3 by the conversion.  4096 rows in chunks of 512 over 4k to 8k keys, 16/2
+// Bound by the chain of the warps that bring the keys: 2800 cycles a tile (loads
+// issued 1100, stores and fence 450, the pair's barrier 600, eight MMAs 500;
+// the softmax takes 1900), 2400 with two CTAs on an SM; in e4m3 the conversion
+// is in it, too.  4096 rows in chunks of 512 over 4k to 8k keys, 16/2
 // heads of 128: 411 us in bf16 (about 470 TFLOP/s without P's second part), 483 in
 // e4m3; 2214 by the kernel for single tokens.  P through shared memory and one
 // place for K and V: 475; values transposed on the way to a K-major operand: 843.
