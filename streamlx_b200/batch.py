@@ -288,7 +288,8 @@ class BatchDecoder:
         if from_last:
             at, slot = (torch.tensor(v, device=dev) for v in zip(*from_last))
             tok[at] = self.last[slot]
-        x = self._forward(tok, plan)
+        used = max(s for s, n in enumerate(n_new) if n > 0) + 1
+        x = self._forward(tok, plan, used)
         if not picking:
             self._check()
             return {}
@@ -301,8 +302,9 @@ class BatchDecoder:
                   self.cfg.trunk_bits, x, self.logits, self.status)
         return self._pick(slots, masks)
 
-    def _forward(self, tok, plan) -> torch.Tensor:
-        """Hidden rows (after the final norm) of the step's tokens."""
+    def _forward(self, tok, plan, n_slots: int) -> torch.Tensor:
+        """Hidden rows (after the final norm) of the step's tokens, which
+        belong to the first ``n_slots`` slots."""
         m, cfg, dev, st = self.model, self.cfg, self.device, self.status
         T, H, hd, bits = tok.shape[0], cfg.hidden, cfg.head_dim, cfg.trunk_bits
         bf = dict(dtype=torch.bfloat16, device=dev)
@@ -316,6 +318,8 @@ class BatchDecoder:
         scores = torch.empty(T, cfg.top_k, dtype=torch.float32, device=dev)
         scratch = torch.zeros(L.router_scratch_bytes(T, cfg.n_experts),
                               dtype=torch.uint8, device=dev)
+        # (the attention goes by the rows that a request of its table has)
+        table = self.cache.table[:n_slots]
         delta = None
         for i, la in enumerate(m.layers):
             pages, scale = self.cache.pages[i], self.cache.kv_scale[i]
@@ -324,7 +328,7 @@ class BatchDecoder:
             q = ops.paged_append(qkv, pages, plan.slot, plan.pos, cfg.heads,
                                  la.q_norm, la.k_norm, cfg.rms_eps,
                                  m.inv_freq, kv_scale=scale, status=st)
-            ops.paged_attention(q, pages, self.cache.table, plan.pos,
+            ops.paged_attention(q, pages, table, plan.pos,
                                 req=plan.req, kv_scale=scale, out=att,
                                 workspace=work, status=st)
             L.qlinear(la.w_o, H, cfg.heads * hd, bits, att, o, st, T=T)

@@ -938,3 +938,35 @@ def test_steps_together(dtype):
         assert ((got - k).abs() <= 2.0 ** (-8 if dtype == BF else -4)
                 * k.abs() + 1e-3).all()
     ops.check_status(torch.device("cuda", torch.cuda.current_device()))
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_attention_chunks_as_single_rows(seed):
+    """Random chunks against the same rows as requests of one row each (the
+    other kernel), and the same bits twice."""
+    g = np.random.default_rng(seed)
+    for _ in range(25):
+        G, nkv = int(g.integers(1, 17)), int(g.choice([1, 2, 3, 8]))
+        hd, page = int(g.choice([64, 128])), int(g.choice([16, 32, 64, 256]))
+        dtype = BF if g.random() < 0.5 else E4
+        lens = [int(n) for n in g.integers(1, int(g.choice([80, 700, 2500])),
+                                           int(g.integers(1, 6)))]
+        host, dev = dev_cache(lens, nkv, hd, page, dtype, seed=seed)
+        req, pos = [], []
+        while len(req) < g.choice([60, 200, 600]):
+            i = int(g.integers(0, len(lens)))
+            n = min(lens[i], int(g.choice([1, 5, 20, 64, 128, 300])))
+            at = int(g.integers(0, lens[i] - n + 1))
+            req += [i] * n + [-1] * 2
+            pos += list(range(at, at + n)) + [-1] * 2
+        q = queries(len(req), G * nkv, hd)
+        out, st = run_attention(q, dev, req, pos)
+        assert st == 0 and torch.equal(out, run_attention(q, dev, req, pos)[0])
+        rows = torch.tensor(req).clamp(min=0)
+        one, st = run_attention(q, (dev[0], dev[1],
+                                    dev[2][rows.cuda()].contiguous()), None,
+                                pos)
+        # both within their bound of the formula: half a bf16 step each, and
+        # what the weights' two parts and fp32 sums leave of the row's size
+        lim = 2.0 ** -7 * one.abs() + 1e-3 * one.abs().amax(-1, keepdim=True)
+        assert st == 0 and ((out - one).abs() <= lim + 1e-4).all()
