@@ -64,8 +64,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   constexpr int KB = HD / 64 * kTileKeys * 128;   // K likewise
   constexpr int VB = KB;                          // V likewise
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_q, bar_k, bar_v, bar_done;
-  __shared__ __align__(8) uint64_t bar_s[2], bar_p[2], bar_o[2];  // by tile's parity
+  __shared__ __align__(8) uint64_t bar_q, bar_done;
+  // by the tile's parity: a warp that runs a tile ahead meets the other barrier
+  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_p[2], bar_o[2];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ int s_keys[kTileM], s_req[kTileM];
@@ -79,10 +80,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const int kh = item % nkv, row0 = item / nkv * rpb;
   if (tid == 0) {
     mbar_init(&bar_q, 128);
-    mbar_init(&bar_k, 64);
-    mbar_init(&bar_v, 64);
     mbar_init(&bar_done, 2);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_k[i], 64);
+      mbar_init(&bar_v[i], 64);
       mbar_init(&bar_s[i], 1);
       mbar_init(&bar_p[i], 128);
       mbar_init(&bar_o[i], 1);
@@ -431,11 +432,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         if (!ok) break;
         store(b);
         fence_proxy_async();
-        mbar_arrive(is_v ? &bar_v : &bar_k);
+        mbar_arrive(is_v ? &bar_v[b] : &bar_k[b]);
         if (is_v) {
           if (tl + 1 < gr.t1) fetch(tl + 1, page);
           page = page_at(tl + 2);
-          if (t == 0 && wait(&bar_p[b], it >> 1) && wait(&bar_v, it)) {
+          if (t == 0 && wait(&bar_p[b], it >> 1) && wait(&bar_v[b], it >> 1)) {
             tc_fence_after();
             // (descriptors count in 16 bytes)
 #pragma unroll
@@ -449,7 +450,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             tc_commit(&bar_o[b]);
           }
         } else {
-          if (t == 0 && (tl > gr.t0 || wait(&bar_q, grp)) && wait(&bar_k, it) &&
+          // (one thread for all of them: it meets every group's bar_q in turn)
+          if (t == 0 && (tl > gr.t0 || wait(&bar_q, grp)) && wait(&bar_k[b], it >> 1) &&
               (it < 2 || wait(&bar_o[b], (it >> 1) - 1))) {
             tc_fence_after();
 #pragma unroll
