@@ -1,5 +1,7 @@
 // Attention of prompt chunks over a paged key-value cache (sm_100a): many rows
 // of a request at a time, on the 5th-generation tensor cores.
+#include <algorithm>
+
 #include "slx_paged.cuh"
 #include "slx_tc.cuh"
 
@@ -548,11 +550,15 @@ int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   const int cols = rpb * G;
   const long long items = (long long)((a.T + rpb - 1) / rpb) * nkv;
   if (items > 0x7fffffff / kTileSplits) return SLX_ERR_UNSUPPORTED;
-  // splits that fill the device, of four tiles and more in the longest request
+  // splits of four tiles and more in the longest request up to two CTAs per SM,
+  // of two up to one (64 rows over 600 keys, 24/4 heads: 20 -> 17 us; 320 rows over
+  // 200 to 1500, 8/8, has the four: 19, by two 21)
   const long long tiles = ((long long)a.max_pages * a.kv.page_size + kTileKeys - 1) / kTileKeys;
-  int nsplit = (int)(items < kTileCtas ? kTileCtas / items : 1);
-  if (nsplit > kTileSplits) nsplit = kTileSplits;
-  if (nsplit > tiles / 4) nsplit = tiles < 8 ? 1 : (int)(tiles / 4);
+  auto splits = [&](int ctas, int least) {
+    const long long n = std::min(ctas / items, tiles / least);
+    return (int)std::max(1LL, std::min(n, (long long)kTileSplits));
+  };
+  const int nsplit = std::max(splits(kTileCtas, 4), splits(kTileCtas / 2, 2));
   TileWork ws;
   ws.o = reinterpret_cast<float*>(a.ws);
   ws.ml = reinterpret_cast<float2*>(ws.o + (size_t)items * nsplit * cols * hd);
