@@ -416,10 +416,13 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // V pairs two keys per register (byte permutes); S^T's accumulators become
 // P^T's operand by movmatrix.
 //
-// P is rounded to two 16-bit parts (hi + lo: 16 bits or more in all), so the
-// only rounding of note is the output's.  E4m3 keys and values become fp16
-// exactly; q becomes fp16 times a power of two per head that puts its largest
-// element at 2^12 .. 2^13 (exact down to 2^-26 of it).
+// P is rounded to two 16-bit parts, hi + lo.  For bf16 pages they are bf16: 16
+// bits of any weight, so the only rounding of note is the output's.  For e4m3
+// pages they are fp16, whose range P is shifted to the top of: the greatest
+// weight is 2^15, one of 2^-29 of it still has 11 bits, and the least step is
+// 2^-39 of it, so a result is off by 2^-40 sum |v| at most.  E4m3 keys and values
+// become fp16 exactly; q becomes fp16 times a power of two per head that puts
+// its largest element at 2^12 .. 2^13 (exact down to 2^-26 of it).
 //
 // Work is cut into units of one kv head (16 bf16 or 32 e4m3 keys); every CTA
 // gets an equal share of the list (row group, kv head, unit), whatever the
@@ -435,6 +438,10 @@ constexpr int kPaStages = 2;  // of a warp's ring
 constexpr int kPaSwitch = 8;  // units
 // 16-key halves of a unit: as many bytes in flight either way
 constexpr int pa_halves(bool e4m3) { return e4m3 ? 2 : 1; }
+// P and its sum are 2^kPaUp times the softmax's (the quotient is not): with fp16
+// parts as high as its range of 65504 allows
+template <bool E4M3>
+constexpr float kPaUp = E4M3 ? 15.f : 0.f;
 
 struct PaWork {       // workspace of one call
   int4* desc;         // [n] split (group, kv head): first, last CTA, row, head
@@ -988,14 +995,14 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             mx = fmaxf(mx, m[nt][i]);
-            const float ms = mx == -INFINITY ? 0.f : mx;
+            const float ms = mx == -INFINITY ? 0.f : mx, mt = ms - kPaUp<E4M3>;
             f[i] = exp2_fast(m[nt][i] - ms);
             m[nt][i] = mx;
             float sum = 0.f;
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-              s[nt][h][i] = exp2_fast(s[nt][h][i] - ms);
-              s[nt][h][i + 2] = exp2_fast(s[nt][h][i + 2] - ms);
+              s[nt][h][i] = exp2_fast(s[nt][h][i] - mt);
+              s[nt][h][i + 2] = exp2_fast(s[nt][h][i + 2] - mt);
               sum += s[nt][h][i] + s[nt][h][i + 2];
             }
             l[nt][i] = l[nt][i] * f[i] + sum;

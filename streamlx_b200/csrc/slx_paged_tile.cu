@@ -12,10 +12,13 @@ namespace slx {
 //   S [128 x 64] = Q K^T,   O [128 x hd] += P V     (tcgen05.mma, M = 128)
 // with S (twice) and O in TMEM.  A column's lane holds it alone, so maximum and
 // sum need no exchange.  P takes the place of its scores in TMEM, the second
-// product's first operand, as two 16-bit parts, hi + lo, both multiplied: 16
-// bits or more, as in the kernel for single tokens.  O is scaled only when a
-// column's maximum has grown by 2^8 (P and the sum stay far inside fp32 and fp16
-// until then).  K and V lie in shared memory as their pages have them, rows of
+// product's first operand, as two 16-bit parts, hi + lo, both multiplied, with
+// the bits that they have in the kernel for single tokens.  For bf16 pages O is
+// scaled only when a column's maximum has grown by 2^8 (P and the sum stay far
+// inside bf16's and fp32's range until then); for e4m3 pages whenever it grows,
+// because P takes all of fp16's range (8/8 heads of 64, 512 rows in chunks of 64:
+// 37 us; 34 with 2^8 of it left for growth, where weights below 2^-32 are lost).
+// K and V lie in shared memory as their pages have them, rows of
 // 64 dims swizzled over 128 bytes: K-major for S, and for P V with the dims
 // inside (the descriptor's other order), so neither is transposed.  E4m3 keys
 // and values become fp16 on the way (exact), q a power of two times fp16.
@@ -40,7 +43,12 @@ constexpr int kTileThreads = 256;
 constexpr int kTileTmem = 256;    // S twice, O
 constexpr int kTileCtas = 296;    // two per SM
 constexpr int kTileSplits = 8;    // parts of a row at most
-constexpr float kTileSlack = 8.f; // a maximum may grow by 2^8 before O is scaled
+// A column's maximum may grow by 2^kTileSlack before O is scaled; P and its sum
+// are 2^kTileUp times the softmax's (the quotient is not).
+template <bool E4M3>
+constexpr float kTileSlack = E4M3 ? 0.f : 8.f;
+template <bool E4M3>
+constexpr float kTileUp = E4M3 ? 15.f : 0.f;
 
 struct TileWork {
   float* o;      // [items][splits][cols][hd]
@@ -225,9 +233,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               r[i][j] = __float_as_uint(s);
               mx = fmaxf(mx, s);
             }
-          const bool more = mx > m + kTileSlack;
+          const bool more = mx > m + kTileSlack<E4M3>;
           const float top = more ? mx : m, ms = top == -INFINITY ? 0.f : top;
-          const float f = more ? exp2_fast(m - ms) : 1.f;
+          const float f = more ? exp2_fast(m - ms) : 1.f, mt = ms - kTileUp<E4M3>;
           m = top;
           l *= f;
           if (t > gr.t0 && __any_sync(0xffffffffu, more)) {
@@ -252,8 +260,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float p0 = exp2_fast(__uint_as_float(r[i][2 * j]) - ms);
-              const float p1 = exp2_fast(__uint_as_float(r[i][2 * j + 1]) - ms);
+              const float p0 = exp2_fast(__uint_as_float(r[i][2 * j]) - mt);
+              const float p1 = exp2_fast(__uint_as_float(r[i][2 * j + 1]) - mt);
               l += p0 + p1;
               if constexpr (!E4M3) {
                 hi[j] = pack_bf16(p0, p1);

@@ -970,3 +970,50 @@ def test_attention_chunks_as_single_rows(seed):
         # what the weights' two parts and fp32 sums leave of the row's size
         lim = 2.0 ** -7 * one.abs() + 1e-3 * one.abs().amax(-1, keepdim=True)
         assert st == 0 and ((out - one).abs() <= lim + 1e-4).all()
+
+
+# -------------------------------------------------- small weights, e4m3 --
+
+def sink_cache(n, n_kv, hd, dtype):
+    """One request whose first key is far above the others, which are zero,
+    and has a value of zero: all of the result is what the others weigh."""
+    scale = torch.tensor([[1.0] * n_kv, [0.02] * n_kv])
+    pages, sc, table = P.make_cache([n], n_kv, hd, 64, dtype, seed=41,
+                                    scale=scale)
+    x = pages.float()
+    x[:, 0] = torch.where(torch.isnan(x[:, 0]), x[:, 0], 0.0)
+    at = int(table[0, 0])
+    x[at, 0, :, 0], x[at, 1, :, 0] = 8.0, 0.0
+    pages = x.to(dtype)
+    return (pages, sc, table), (pages.cuda(), None if sc is None else sc.cuda(),
+                                table.cuda())
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("bits", [16.6, 24.6, 27.3, 30.4])
+@pytest.mark.parametrize("nq,nkv,hd,n,rows", [
+    (16, 2, 128, 400, 1), (16, 2, 128, 20000, 1), (24, 4, 64, 3000, 3),
+    (16, 2, 128, 4000, 80),                 # the kernel for chunks, in parts
+    (8, 8, 64, 2600, 2432)])                # and in one
+def test_attention_small_weights(nq, nkv, hd, n, rows, bits, dtype):
+    """Thousands of keys whose weights are 2^-bits of the first one's.
+
+    The bound is the formula's, and for e4m3 pages half of the weights' fp16
+    step, 2^-24 of 2^15, for every key: 2^-40 sum |v| (the greatest weight is
+    at most 1)."""
+    host, dev = sink_cache(n, nkv, hd, dtype)
+    q = torch.ones(rows, nq, hd, dtype=BF)
+    scale = bits * float(np.log(2.0)) / (8 * hd)
+    pos = list(range(n - rows, n))
+    out, st = run_attention(q, dev, [0] * rows, pos, scale)
+    assert st == 0 and torch.isfinite(out).all()
+    some = sorted({0, rows - 1, *range(0, rows, max(1, rows // 40))})
+    want, bound = P.attention(q[some], host[0], host[1], host[2],
+                              [0] * len(some), [pos[r] for r in some], 64,
+                              scale)
+    if dtype == E4:
+        V = P.dense(host[0], host[1], host[2], 0, n, 64)[1]     # [kv, n, hd]
+        step = 2.0 ** -40 * V.abs().sum(1)
+        bound = bound + step.repeat_interleave(nq // nkv, 0)
+    err = (out[some].double() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
