@@ -524,9 +524,10 @@ size_t slx_paged_attn_workspace_bytes(int T, int n_q, int n_kv, int head_dim);
 /* Attention of T rows over the pages (GQA, n_q / n_kv <= 16): row t attends
  * positions 0..pos[t] of request req[t] (req NULL: request t).
  * q [T][q_stride] bf16 (n_q heads of head_dim), out [T][n_q * head_dim]
- * bf16.  max_pages * page_size <= 2^30.  A row with pos < 0 gives zeros; a row with req or pos out of range
- * sets *status and gives zeros; keys and values on a page out of range set
- * *status and read as zeros. */
+ * bf16.  max_pages * page_size <= 2^30.  A row with pos < 0 gives zeros; a row
+ * with req or pos out of range sets *status and gives zeros; keys and values on
+ * a page out of range set *status and read as zeros.  Rows of one request are
+ * best side by side: runs of many rows share the keys they read. */
 int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
                           const slx_kv_pages* pages, const int32_t* table,
                           int n_req, int max_pages, const int32_t* req,

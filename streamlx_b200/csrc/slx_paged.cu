@@ -507,9 +507,10 @@ struct PaSeg {
   int row, kh, u0, u1, units, keys, req;
 };
 
-template <int HD, bool E4M3, int NT>
+// REST: behind k_paged_tile, for the rows that it has left.
+template <int HD, bool E4M3, int NT, bool REST>
 __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
-    k_paged_attn(const PagedAttnArgs a, const PaWork ws, int rpb) {
+    k_paged_attn(const PagedAttnArgs a, const PaWork ws, int rpb, const TileWork tile) {
   constexpr int ES = E4M3 ? 1 : 2;       // bytes per element
   constexpr int RB = HD * ES;            // a key's row
   constexpr int KQ = RB / 64;            // 16-byte pieces of a key per lane
@@ -540,6 +541,22 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   const bool by_row = (long long)a.T * nkv <= nw;  // how desc is indexed
   pdl_launch_dependents();
   pdl_wait_primary();
+  if constexpr (REST) {
+    if (tile.n_left) {
+      int any = 0;
+      for (int i = tid; i < tile.n_left; i += kPaThreads) any |= tile.left[i];
+      if (!__syncthreads_or(any)) {
+        if (tid == 0) ws.desc[w] = make_int4(-1, 0, 0, 0);
+        return;
+      }
+    }
+  }
+  // the keys of the group that row t0 + lane leads and that falls to this kernel
+  auto lead = [&](const RowKeys& r, int t0) {
+    const int n = lead_keys(r.keys, r.req, rpb);
+    if constexpr (REST) return in_run(a, t0, tile.least) ? 0 : n;
+    return n;
+  };
   auto units_of = [](int keys) { return (int)(((unsigned)keys + kPaUnit - 1) / kPaUnit); };
   auto weight_of = [&](int keys) { return keys ? units_of(keys) + kPaSwitch : 0; };
   // weights before each of 128 runs of `run` tiles of 32 rows
@@ -549,7 +566,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   long long total;
   if (tiles == 1) {
     rk = row_keys(a, lane);
-    len_l = lead_keys(rk.keys, rk.req, rpb);
+    len_l = lead(rk, 0);
     total = warp_sum(weight_of(len_l)) * nkv;
   } else {
     s_pre[tid + 1] = 0;
@@ -561,7 +578,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
       for (int j = 0; j < B; ++j) r[j] = row_keys(a, (i0 + j) * 32 + lane);
 #pragma unroll
       for (int j = 0; j < B; ++j) {
-        const long long v = warp_sum(weight_of(lead_keys(r[j].keys, r[j].req, rpb)));
+        const long long v = warp_sum(weight_of(lead(r[j], (i0 + j) * 32)));
         if (lane == 0 && i0 + j < tiles)
           atomicAdd(reinterpret_cast<unsigned long long*>(&s_pre[(i0 + j) / run + 1]),
                     (unsigned long long)v);
@@ -605,7 +622,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
       for (;; rb += 32) {
         if (tiles > 1) {
           rk = row_keys(a, rb + lane);
-          len_l = lead_keys(rk.keys, rk.req, rpb);
+          len_l = lead(rk, rb);
         }
         const int n = weight_of(len_l);
         const long long all = warp_sum(n);
@@ -660,7 +677,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
         while (!hit) {  // there is one: x < total
           p.rb += 32;
           const RowKeys r = row_keys(a, p.rb + lane);
-          p.len = lead_keys(r.keys, r.req, rpb);
+          p.len = lead(r, p.rb);
           p.req = r.req;
           hit = __ballot_sync(0xffffffffu, p.len > 0);
         }
@@ -1258,7 +1275,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 64 ? 5 - NT : 4 - NT)
   for (int i = w; i < tiles; i += nw) {
     const int t = i * 32 + lane;
     const RowKeys r = row_keys(a, t);
-    const int n = lead_keys(r.keys, r.req, rpb);
+    const int n = lead(r, i * 32);
     if (by_row && t < a.T && n == 0)
       for (int k = 0; k < nkv; ++k) ws.desc[t * nkv + k] = make_int4(-1, 0, 0, 0);
     const bool idle = t < a.T && r.keys == 0;
@@ -1374,27 +1391,32 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedAttnArgs
 
 namespace {
 
-using AttnKernel = void (*)(PagedAttnArgs, PaWork, int);
+using AttnKernel = void (*)(PagedAttnArgs, PaWork, int, TileWork);
 
-AttnKernel attn_kernel(int hd, bool e4m3, int nt, int* id, size_t* smem) {
+template <bool REST>
+AttnKernel attn_kernel(int i) {
   static const AttnKernel k[8] = {
-      k_paged_attn<64, false, 1>,  k_paged_attn<64, false, 2>,
-      k_paged_attn<64, true, 1>,   k_paged_attn<64, true, 2>,
-      k_paged_attn<128, false, 1>, k_paged_attn<128, false, 2>,
-      k_paged_attn<128, true, 1>,  k_paged_attn<128, true, 2>};
-  const int rb = hd * (e4m3 ? 1 : 2);
-  *id = (hd == 128 ? 4 : 0) + (e4m3 ? 2 : 0) + nt - 1;
+      k_paged_attn<64, false, 1, REST>,  k_paged_attn<64, false, 2, REST>,
+      k_paged_attn<64, true, 1, REST>,   k_paged_attn<64, true, 2, REST>,
+      k_paged_attn<128, false, 1, REST>, k_paged_attn<128, false, 2, REST>,
+      k_paged_attn<128, true, 1, REST>,  k_paged_attn<128, true, 2, REST>};
+  return k[i];
+}
+
+AttnKernel attn_kernel(int hd, bool e4m3, int nt, bool rest, int* id, size_t* smem) {
+  const int rb = hd * (e4m3 ? 1 : 2), i = (hd == 128 ? 4 : 0) + (e4m3 ? 2 : 0) + nt - 1;
+  *id = i + (rest ? 8 : 0);
   // the warps' rings and two warps' accumulators
   *smem = (e4m3 ? (size_t)kPaWarps * kPaStages * 2 * 16 * pa_halves(e4m3) * rb : 0) +
           (size_t)kPaWarps / 2 * nt * (hd / 16) * 512;
-  return k[*id];
+  return rest ? attn_kernel<true>(i) : attn_kernel<false>(i);
 }
 
 constexpr int kPaMaxCtas = 1024;  // CTAs of a launch (workspace size)
 
 // CTAs that fill the current device; 0 on a CUDA error.
 int attn_ctas(AttnKernel k, int id, size_t smem) {
-  static PerDevice known[8];
+  static PerDevice known[16];
   std::atomic<int>& slot = known[id].here();
   int n = slot.load(std::memory_order_relaxed);
   if (!n) {
@@ -1418,14 +1440,19 @@ int attn_rows(int G, int nt) {
   return n;
 }
 
-}  // namespace
-
-// desc | parts' O | parts' (max, sum), for the largest launch
-size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
-  if (T == 0) return 0;
+// desc | parts' O | parts' (max, sum), for the largest launch, or the parts of
+// the kernel for chunks, which are joined before this one's are written
+size_t attn_parts_bytes(int nq, int nkv, int hd) {
   const size_t G = nq / nkv, cols = attn_rows((int)G, 2) * G;
   const size_t n = kPaMaxCtas * (sizeof(int4) + 2 * cols * (hd * sizeof(float) + sizeof(float2)));
   return std::max(n, paged_tile_workspace_bytes(nq, nkv, hd));
+}
+
+}  // namespace
+
+// The parts, and the flags between the two kernels.
+size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
+  return T == 0 ? 0 : attn_parts_bytes(nq, nkv, hd) + kTileFlags * sizeof(int32_t);
 }
 
 int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
@@ -1435,8 +1462,26 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   // in bf16, chunks of 8: 215 -> 109 us; 64 rows, 16/2, chunks of 8: 25 -> 17.
   // Not so for 32 columns (512 rows in chunks of 32, 8/8 heads of 64: 42 -> 53)
   // or 256 in all (16 rows, 16/2: 16 -> 21).
-  if (a.req && paged_tile_rows(a) * G >= 48 && (long long)a.T * a.nq >= 1024)
-    return launch_paged_tile(a, e4m3, s);
+  //
+  // The average does not say which requests have the rows, so that kernel takes
+  // the runs of 32 columns and more and this one what is left of the call (unless
+  // there is one request).  63 requests of one row over 4000 keys beside a chunk
+  // of 512, 24/4 heads of 128 in bf16: 260 us (88 and 82 by themselves; the blocks
+  // of the average's 8 rows fill 48 of 128 columns), 863 by that kernel alone.
+  // Calls with nothing left pay for two empty launches: 5 chunks of 64 rows, 8/8
+  // heads of 64, e4m3: 19.2 -> 22 us, 8 of 512, 16/2 of 128: 412 -> 417.
+  TileWork tile = {};
+  const bool chunks = a.req && paged_tile_rows(a) * G >= 48 && (long long)a.T * a.nq >= 1024;
+  const bool rest = chunks && a.n_req > 1;
+  if (chunks) {
+    tile.o = reinterpret_cast<float*>(a.ws);
+    tile.left = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(a.ws) +
+                                           attn_parts_bytes(a.nq, nkv, a.kv.hd));
+    tile.least = rest ? (31 + G) / G : 0;
+    const int rc = launch_paged_tile(a, e4m3, tile, s);
+    if (rc) return rc;
+    if (!rest) return SLX_OK;
+  }
   // Two column tiles where one row needs them, or where a request has the rows
   // to fill them on average and there is work for the device: the keys are read
   // and turned into operands half as often.  One tile -> two, 24/4 heads of 128
@@ -1445,12 +1490,12 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   // rows in chunks of 8 (half a tile): 45 -> 62, of 16: 43 -> 38; 64 rows: 15.3
   // -> 17.1.
   const int tall = attn_rows(G, 2);
-  const bool many =
-      a.req && tall > attn_rows(G, 1) && a.T / tall >= a.n_req && (long long)a.T * a.nq >= 768;
+  const bool many = !rest && a.req && tall > attn_rows(G, 1) && a.T / tall >= a.n_req &&
+                    (long long)a.T * a.nq >= 768;
   const int nt = G > 8 || many ? 2 : 1;
   int id;
   size_t smem;
-  const AttnKernel k = attn_kernel(a.kv.hd, e4m3, nt, &id, &smem);
+  const AttnKernel k = attn_kernel(a.kv.hd, e4m3, nt, rest, &id, &smem);
   const int full = attn_ctas(k, id, smem);
   if (full < 1) return SLX_ERR_CUDA;
   // no more CTAs than steps (a unit per warp) the rows could fill
@@ -1468,7 +1513,8 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   ws.desc = reinterpret_cast<int4*>(p);
   ws.o = reinterpret_cast<float*>(p + kPaMaxCtas * sizeof(int4));
   ws.ml = reinterpret_cast<float2*>(ws.o + (size_t)kPaMaxCtas * 2 * cols * a.kv.hd);
-  if (launch_k(k, dim3(grid), dim3(kPaThreads), smem, s, a, ws, rpb) != cudaSuccess)
+  if ((rest ? launch_chained(k, dim3(grid), dim3(kPaThreads), smem, s, a, ws, rpb, tile)
+            : launch_k(k, dim3(grid), dim3(kPaThreads), smem, s, a, ws, rpb, tile)) != cudaSuccess)
     return SLX_ERR_CUDA;
   // one CTA per column while they fit the device about twice over
   const unsigned n = (unsigned)(segs <= grid ? segs : grid);

@@ -50,11 +50,6 @@ constexpr float kTileSlack = E4M3 ? 0.f : 8.f;
 template <bool E4M3>
 constexpr float kTileUp = E4M3 ? 15.f : 0.f;
 
-struct TileWork {
-  float* o;      // [items][splits][cols][hd]
-  float2* ml;    // [items][splits][cols] max (log2), sum
-};
-
 // Bits of the block's rows, in four words: the first one set at `from` or
 // behind it (kTileM: none).
 SLX_DEV int next_bit(const uint32_t* m, int from) {
@@ -68,7 +63,7 @@ SLX_DEV int next_bit(const uint32_t* m, int from) {
 
 template <int HD, bool E4M3>
 __global__ void __launch_bounds__(kTileThreads, 2)
-    k_paged_tile(const PagedAttnArgs a, const TileWork ws, int rpb, int nsplit) {
+    k_paged_tile(const PagedAttnArgs a, const TileWork ws) {
   constexpr int ES = E4M3 ? 1 : 2, RB = HD * ES;  // bytes of an element, of a key
   constexpr int QB = HD / 64 * kTileM * 128;      // Q: chunks of 64 dims, swizzled
   constexpr int KB = HD / 64 * kTileKeys * 128;   // K likewise
@@ -81,10 +76,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __shared__ volatile int s_abort;
   __shared__ int s_keys[kTileM], s_req[kTileM];
   __shared__ uint32_t s_start[kTileM / 32], s_stop[kTileM / 32];
+  __shared__ int s_left[kTileM / 32];
   __shared__ int s_odd[kTileM][2];  // by group's first row: keys with odd values
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sQ = base, *sK = sQ + QB, *sV = sK + 2 * KB;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rpb = ws.rpb, nsplit = ws.nsplit;
   const int nkv = a.kv.n_kv, G = a.nq / nkv, ps = a.kv.page_size, sh = a.kv.page_shift;
   const int split = blockIdx.x % nsplit, item = blockIdx.x / nsplit;
   const int kh = item % nkv, row0 = item / nkv * rpb;
@@ -108,15 +105,19 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     tc_alloc(&s_tmem, kTileTmem);
     tc_relinquish();
   }
-  // the block's rows, and where its groups (rows of one request) begin and end
+  // the block's rows, and where its groups (rows of one request) begin and end;
+  // with the other kernel behind this one, rows of short runs and idle ones are
+  // left to it
   if (tid < kTileM) {
     const RowKeys r = row_keys(a, tid < rpb ? row0 + tid : a.T);
-    s_keys[tid] = r.keys;
+    const bool mine = !ws.least || in_run(a, row0 + 32 * warp, ws.least);
+    s_keys[tid] = mine ? r.keys : 0;
     s_req[tid] = r.req;
     s_odd[tid][0] = 0x7fffffff;
     s_odd[tid][1] = -1;
-    if (split == 0 && kh == 0 && r.keys == 0 && r.pos >= 0 && tid < rpb)
+    if (!ws.least && split == 0 && kh == 0 && r.keys == 0 && r.pos >= 0 && tid < rpb)
       set_status(a.status, SLX_ERR_OUT_OF_RANGE);
+    s_left[warp] = __any_sync(0xffffffffu, tid < rpb && row0 + tid < a.T && s_keys[tid] == 0);
   }
   __syncthreads();
   if (tid < kTileM) {
@@ -133,6 +134,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __syncthreads();
   tc_fence_after();
   pdl_launch_dependents();
+  if (tid == 0 && split == 0 && kh == 0 && ws.n_left)
+    ws.left[row0 / rpb] = s_left[0] | s_left[1] | s_left[2] | s_left[3];
   const uint32_t tmem = s_tmem;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_wait(bar, parity & 1, a.status) && !s_abort) return true;
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     // ------------------------------------------------ softmax, a column each --
     const int ri = tid / G, hh = kh * G + tid % G;
     const uint32_t t_lane = tmem + ((uint32_t)(32 * warp) << 16), t_o = t_lane + 2 * kTileKeys;
-    if (split == 0 && ri < rpb && row0 + ri < a.T && s_keys[ri] == 0) {
+    if (!ws.least && split == 0 && ri < rpb && row0 + ri < a.T && s_keys[ri] == 0) {
       uint4* o = reinterpret_cast<uint4*>(a.out + ((size_t)(row0 + ri) * a.nq + hh) * HD);
       for (int i = 0; i < HD / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
     }
@@ -496,19 +499,21 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 
 // A warp per (row, q head): its splits' parts in the order of the keys.
 template <int HD>
-__global__ void __launch_bounds__(256) k_paged_tile_join(const PagedAttnArgs a, const TileWork ws,
-                                                         int rpb, int nsplit) {
+__global__ void __launch_bounds__(256) k_paged_tile_join(const PagedAttnArgs a, const TileWork ws) {
   pdl_launch_dependents();
   pdl_wait_primary();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, rpb = ws.rpb, nsplit = ws.nsplit;
   const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (id >= (long long)a.T * a.nq) return;
   const int row = (int)(id / a.nq), hh = (int)(id % a.nq), G = a.nq / a.kv.n_kv;
-  if (row_keys(a, row).keys == 0) return;  // zeros already
   const int col = row % rpb * G + hh % G;
   const size_t item = (size_t)(row / rpb) * a.kv.n_kv + hh / G;
   auto part = [&](int i) { return (item * nsplit + i) * (rpb * G) + col; };
+  // (requested with the row; of no use where the row has no parts)
   const float2 ml = lane < nsplit ? ws.ml[part(lane)] : make_float2(-INFINITY, 0.f);
+  const RowKeys r = row_keys(a, row);
+  const bool mine = !ws.least || in_run(a, row, ws.least);  // (lane 0: this row)
+  if (r.keys == 0 || !__shfl_sync(0xffffffffu, mine, 0)) return;
   float4 v[4], o = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool on = lane < HD / 4;
   float M = ml.x;
@@ -553,10 +558,11 @@ int paged_tile_rows(const PagedAttnArgs& a) {
   return each < most ? (each > 0 ? each : 1) : most;
 }
 
-int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
+// Lays out the parts behind ws.o, fills in how the rows are cut, and joins them.
+int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStream_t s) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv, hd = a.kv.hd, rpb = paged_tile_rows(a);
-  const int cols = rpb * G;
-  const long long items = (long long)((a.T + rpb - 1) / rpb) * nkv;
+  const int cols = rpb * G, blocks = (a.T + rpb - 1) / rpb;
+  const long long items = (long long)blocks * nkv;
   if (items > 0x7fffffff / kTileSplits) return SLX_ERR_UNSUPPORTED;
   // splits of four tiles and more in the longest request up to two CTAs per SM,
   // of two up to one (64 rows over 600 keys, 24/4 heads: 20 -> 17 us; 320 rows over
@@ -567,10 +573,11 @@ int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
     return (int)std::max(1LL, std::min(n, (long long)kTileSplits));
   };
   const int nsplit = std::max(splits(kTileCtas, 4), splits(kTileCtas / 2, 2));
-  TileWork ws;
-  ws.o = reinterpret_cast<float*>(a.ws);
   ws.ml = reinterpret_cast<float2*>(ws.o + (size_t)items * nsplit * cols * hd);
-  using Kernel = void (*)(PagedAttnArgs, TileWork, int, int);
+  ws.rpb = rpb;
+  ws.nsplit = nsplit;
+  ws.n_left = ws.least && blocks <= kTileFlags ? blocks : 0;
+  using Kernel = void (*)(PagedAttnArgs, TileWork);
   const Kernel k = hd == 128 ? (e4m3 ? k_paged_tile<128, true> : k_paged_tile<128, false>)
                              : (e4m3 ? k_paged_tile<64, true> : k_paged_tile<64, false>);
   // Q, two tiles of K and of V, and what aligns them
@@ -583,13 +590,13 @@ int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
       return SLX_ERR_CUDA;
     slot.store(1, std::memory_order_relaxed);
   }
-  if (launch_k(k, dim3((unsigned)(items * nsplit)), dim3(kTileThreads), smem, s, a, ws, rpb,
-               nsplit) != cudaSuccess)
+  if (launch_k(k, dim3((unsigned)(items * nsplit)), dim3(kTileThreads), smem, s, a, ws) !=
+      cudaSuccess)
     return SLX_ERR_CUDA;
   if (nsplit == 1) return SLX_OK;
   const long long warps = (long long)a.T * a.nq;
   return launch_chained(hd == 128 ? k_paged_tile_join<128> : k_paged_tile_join<64>,
-                        dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a, ws, rpb, nsplit) ==
+                        dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a, ws) ==
                  cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
 }
 

@@ -1017,3 +1017,86 @@ def test_attention_small_weights(nq, nkv, hd, n, rows, bits, dtype):
         bound = bound + step.repeat_interleave(nq // nkv, 0)
     err = (out[some].double() - want).abs()
     assert (err <= bound).all(), float((err / bound).max())
+
+
+# ------------------------------------- chunks beside single tokens --
+
+def graph_us(call, n=10):
+    """Time of one of n calls in a graph, the least of some replays."""
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for _ in range(n):
+            call()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in "ab")
+    best = float("inf")
+    for _ in range(10):
+        a.record()
+        g.replay()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1000 / n)
+    return best
+
+
+def attention_us(lens, rows, nq, nkv, hd, dtype, idle=0):
+    """Of the last rows[i] tokens of every request, then `idle` padding rows
+    (the pages' content is of no matter here)."""
+    need = [P.pages_for(n, 64) for n in lens]
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = torch.arange(at, at + n)
+        at += n
+    pages = torch.zeros(at, 2, nkv, 64, hd, device="cuda").to(dtype)
+    sc = torch.ones(2, nkv, device="cuda") if dtype == E4 else None
+    req, pos = chunk_rows(lens, [n - r for n, r in zip(lens, rows)])
+    req, pos = (torch.tensor(v + [-1] * idle, dtype=torch.int32).cuda()
+                for v in (req, pos))
+    q = torch.ones(len(req), nq, hd, dtype=BF, device="cuda")
+    table = table.cuda()
+    return graph_us(lambda: ops.paged_attention(q, pages, table, pos, req=req,
+                                                kv_scale=sc))
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_mixed_rows_cost_their_parts(dtype):
+    """A prompt chunk beside decoding requests, and a call that is padding for
+    the most part, against the parts by themselves (the least of ten replays):
+    the chunk's blocks hold 48 of 128 columns at least, so it may take 128 / 48
+    of its time; 25 us for up to four launches more."""
+    heads = (24, 4, 128, dtype)
+    decode = attention_us([4000] * 63, [1] * 63, *heads)
+    chunk = attention_us([4000], [512], *heads)
+    mixed = attention_us([4000] * 64, [1] * 30 + [512] + [1] * 33, *heads)
+    assert mixed <= decode + 128 / 48 * chunk + 25, (mixed, decode, chunk)
+    heads = (16, 2, 128, dtype)
+    decode = attention_us([30000] * 7, [1] * 7, *heads)
+    chunk = attention_us([2000], [64], *heads)
+    mixed = attention_us([2000] + [30000] * 7, [64] + [1] * 7, *heads)
+    assert mixed <= decode + 128 / 48 * chunk + 25, (mixed, decode, chunk)
+    few = attention_us([30000] * 3, [1] * 3, *heads)
+    padded = attention_us([30000] * 3 + [1], [1] * 3 + [0], *heads, idle=61)
+    assert padded <= few + 25, (padded, few)
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+@pytest.mark.parametrize("nq,nkv,hd", [(24, 4, 128), (8, 8, 64), (32, 2, 64),
+                                       (16, 2, 128), (13, 1, 128), (2, 1, 64)])
+def test_attention_runs_of_every_length(nq, nkv, hd, dtype):
+    """Chunks of 1 to 70 rows beside each other, in an order that puts their
+    ends at any place of the blocks, idle rows between and inside them."""
+    g = np.random.default_rng(nq + hd)
+    each = [int(n) for n in g.permutation([*range(1, 40), 47, 48, 49, 63, 64,
+                                           65, 70] + [1] * 12)]
+    lens = [n + int(g.integers(0, 150)) for n in each]
+    req, pos = [], []
+    for i, (n, r) in enumerate(zip(lens, each)):
+        req += [i] * r + [-1] * int(g.integers(0, 2))
+        pos += list(range(n - r, n)) + [-1] * (len(req) - len(pos) - r)
+    for r in g.integers(0, len(req), 5):
+        pos[r] = -1
+    host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=nq)
+    out = check_attention(queries(len(req), nq, hd), host, dev, req, pos)
+    assert all((out[r] == 0).all() for r in range(len(req)) if pos[r] < 0)
