@@ -352,10 +352,14 @@ class BatchDecoder:
             kw = {name: torch.tensor([getattr(u, name) for u in rules],
                                      dtype=torch.float32).to(dev)
                   for name in ("repetition", "frequency", "presence")}
-            kw["history"] = self.history[at, :max(n_hist)].contiguous()
-            kw["n_prompt"] = torch.tensor([len(r.prompt) for r in reqs],
-                                          dtype=torch.int32).to(dev)
-            kw["n_history"] = torch.tensor(n_hist, dtype=torch.int32).to(dev)
+            # (no history of the others: they may be longer than MAX_HISTORY)
+            said = [u.penalises for u in rules]
+            n = [h if p else 0 for h, p in zip(n_hist, said)]
+            kw["history"] = self.history[at, :max(n)].contiguous()
+            kw["n_prompt"] = torch.tensor(
+                [len(r.prompt) if p else 0 for r, p in zip(reqs, said)],
+                dtype=torch.int32).to(dev)
+            kw["n_history"] = torch.tensor(n, dtype=torch.int32).to(dev)
         if any(u.bias for u in rules):
             b = [list(u.bias.items()) for u in rules]
             start = np.cumsum([0] + [len(e) for e in b]).astype(np.int32)

@@ -1,0 +1,52 @@
+"""Bookkeeping of the batched decoder that needs no GPU: what it takes, what it
+refuses, and what it hands to the kernels' front ends."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from streamlx_b200 import batch, ops
+from streamlx_b200.batch import BatchDecoder, LogitRules
+
+VOCAB = 50
+
+
+def decoder(**kw):
+    """A decoder over a model of which only the sizes are looked at."""
+    cfg = SimpleNamespace(has_trunk=True, head_dim=64, heads=4, kv_heads=2,
+                          layers=2, vocab=VOCAB)
+    layers = [SimpleNamespace(k_norm=torch.ones(64)) for _ in range(2)]
+    model = SimpleNamespace(cfg=cfg, ep=None, device=torch.device("cpu"),
+                            layers=layers)
+    args = dict(max_requests=3, max_tokens=64, page_size=16)
+    args.update(kw)
+    return BatchDecoder(model, **args)
+
+
+def test_history_of_penalised_requests_alone(monkeypatch):
+    """The history that goes to the kernel is as wide as the longest request
+    with penalties, and other requests' rows of it count for nothing: the
+    longest of all may be longer than penalties reach."""
+    monkeypatch.setattr(batch, "MAX_HISTORY", 30)
+    dec = decoder()
+    dec.submit(list(range(40)), 5)                       # longer than that
+    dec.submit([1, 2, 3], 5, LogitRules(presence=1.0))
+    dec.submit([4, 5], 5, LogitRules(bias={3: 1.0}))
+    dec._admit()
+    dec.slots[1].out = [7, 8]
+    seen = {}
+
+    def process(logits, **kw):
+        seen.update(kw)
+        return torch.tensor([10, 11, 12], dtype=torch.int32)
+
+    monkeypatch.setattr(ops, "process_logits", process)
+    dec.logits = torch.zeros(3, VOCAB)
+    assert dec._pick((0, 1, 2), {}) == {0: 10, 1: 11, 2: 12}
+    assert seen["history"].shape == (3, 5)
+    assert seen["n_history"].tolist() == [0, 5, 0]
+    assert seen["n_prompt"].tolist() == [0, 3, 0]
+    # the picked tokens stand at their own places all the same
+    assert dec.history[0, 40] == 10 and dec.history[1, 5] == 11
+    assert dec.history[2, 2] == 12
