@@ -384,9 +384,7 @@ class BatchDecoder:
         for s, r, t in zip(slots, reqs, got):
             r.out.append(t)
             if t < 0 or t == r.eos or len(r.out) >= r.max_new:
-                self._reserved -= self._pages(r)
-                self.slots[s] = None
-                self._gone.add(s)
+                self._end(s)
         return {r.rid: t for r, t in zip(reqs, got)}
 
     def _check(self) -> None:
@@ -402,7 +400,9 @@ class BatchDecoder:
                  eos: int | None = None) -> list[list[int]]:
         """Every prompt to its end; ``rules``: one LogitRules, or one per
         prompt.  A mask that allows nothing ends a request without a token.
-        Not while submitted requests run: their tokens come from ``step``."""
+        Not while submitted requests run: their tokens come from ``step``.
+        When it raises (a prompt that is refused, a mask that raises) none of
+        its requests stays."""
         if self.busy:
             raise RuntimeError("generate: submitted requests are running, "
                                "their tokens come from step")
@@ -410,14 +410,32 @@ class BatchDecoder:
             rules = [rules] * len(prompts)
         if len(rules) != len(prompts):
             raise ValueError("one LogitRules per prompt")
-        ids = [self.submit(p, max_new, r, eos) for p, r in zip(prompts, rules)]
-        out: dict = {i: [] for i in ids}
-        while self.busy:
-            for rid, t in self.step().items():
-                if t >= 0:
-                    out[rid].append(t)
+        ids: list[int] = []
+        try:
+            for p, r in zip(prompts, rules):
+                ids.append(self.submit(p, max_new, r, eos))
+            out: dict = {i: [] for i in ids}
+            while self.busy:
+                for rid, t in self.step().items():
+                    if t >= 0:
+                        out[rid].append(t)
+        except BaseException:
+            self._withdraw(set(ids))
+            raise
         self.release()
         return [out[i] for i in ids]
+
+    def _withdraw(self, ids: set[int]) -> None:
+        """Drop requests; the running ones' pages go back with the next step."""
+        self._queue = deque(r for r in self._queue if r.rid not in ids)
+        for s, r in enumerate(self.slots):
+            if r is not None and r.rid in ids:
+                self._end(s)
+
+    def _end(self, s: int) -> None:
+        self._reserved -= self._pages(self.slots[s])
+        self.slots[s] = None
+        self._gone.add(s)
 
     def release(self) -> None:
         """Hand the finished requests' pages back now (a step does, too)."""

@@ -50,3 +50,47 @@ def test_history_of_penalised_requests_alone(monkeypatch):
     # the picked tokens stand at their own places all the same
     assert dec.history[0, 40] == 10 and dec.history[1, 5] == 11
     assert dec.history[2, 2] == 12
+
+
+def idle(dec):
+    return (not dec.busy and dec._reserved == 0 and
+            all(r is None for r in dec.slots))
+
+
+def test_refused_generate_leaves_nothing_queued():
+    dec = decoder()
+    for prompts, rules in (([[1], [VOCAB]], None), ([[1], [2] * 64], None),
+                           ([[1], []], None), ([[1], [2]], [None])):
+        with pytest.raises(ValueError):
+            dec.generate(prompts, 2, rules)
+        assert idle(dec)
+    with pytest.raises(ValueError):
+        dec.generate([[1], [2]], 2, [None, LogitRules(bias={VOCAB: 1.0})])
+    assert idle(dec)
+
+
+def test_failed_generate_takes_its_requests_back():
+    """A step that raises before it changed anything (a mask that raises):
+    generate's requests go, running and waiting ones, and nobody else's are
+    touched."""
+    dec = decoder(max_requests=2)
+    steps = []
+
+    def step():
+        dec._admit()
+        steps.append([r.rid for r in dec.slots if r is not None])
+        for r in dec.slots:
+            r.fed = len(r.prompt)
+        if len(steps) == 2:
+            raise KeyError("no such state")
+        return {r.rid: 1 for r in dec.slots}
+
+    dec.step = step
+    with pytest.raises(KeyError):
+        dec.generate([[1], [2], [3]], 4)
+    assert steps == [[0, 1], [0, 1]] and idle(dec)
+    assert dec._gone == {0, 1}          # their pages go back with the next step
+    rid = dec.submit([1], 2)
+    with pytest.raises(RuntimeError):
+        dec.generate([[1]], 2)          # not beside submitted ones
+    assert [r.rid for r in dec._queue] == [rid]

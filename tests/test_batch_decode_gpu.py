@@ -242,3 +242,29 @@ def test_failed_masks_and_steps(tiny):
     with pytest.raises(RuntimeError, match="lost"):
         dec.step()
     reader.close()
+
+
+def test_generate_after_a_failed_one(tiny):
+    """A generate that raises in its middle leaves nothing behind: the same
+    decoder, whose pages hold two requests at most, generates as before."""
+    cfg, model, reader = load(tiny["tiny_dec"])
+    rng = np.random.default_rng(11)
+    prompts = [rng.integers(0, cfg.vocab, n).tolist() for n in (9, 20, 5)]
+    want = model.generate_batch(prompts, 6)
+    dec = BatchDecoder(model, max_requests=2, max_tokens=32, page_size=16,
+                       prompt_chunk=4)
+
+    def mask(out):
+        if len(out) == 2:
+            raise KeyError("no such state")
+
+    for rules in ([None, None, LogitRules(mask=mask)],
+                  [LogitRules(mask=mask), None, None]):
+        with pytest.raises(KeyError):
+            dec.generate(prompts, 6, rules)
+        assert not dec.busy
+        with pytest.raises(ValueError):
+            dec.generate([prompts[0], [cfg.vocab]], 6)
+        assert dec.generate(prompts, 6) == want
+    assert int(dec.cache.n_free.item()) == dec.cache.n_pages
+    reader.close()
