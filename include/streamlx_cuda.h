@@ -535,6 +535,11 @@ int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
                           void* workspace, size_t workspace_bytes,
                           int32_t* status, void* stream);
 
+/* Kernels that this thread's last slx_paged_attn_decode launched: by its rows
+ * and sizes up to 4 (both kernels for rows, each with its parts' join), 0 when
+ * it had no rows or was refused. */
+int slx_paged_attn_launches(void);
+
 /* What is applied to a step's logits; every pointer may be NULL. */
 typedef struct slx_logit_rules {
   const int32_t* history;    /* [T][history_stride] the row's token ids:

@@ -48,7 +48,7 @@ EXPORTS = (
     "slx_ep_grid", "slx_switchglu_ep", "slx_ep_combine_rmsnorm",
     "slx_ipc_handle", "slx_ipc_open", "slx_ipc_close",
     "slx_paged_plan", "slx_paged_append", "slx_paged_attn_workspace_bytes",
-    "slx_paged_attn_decode", "slx_logits_process",
+    "slx_paged_attn_decode", "slx_paged_attn_launches", "slx_logits_process",
 )
 EP_MAX_RANKS = 8
 
@@ -259,6 +259,8 @@ def lib() -> C.CDLL:
         L.slx_paged_attn_decode.argtypes = [vp, C.c_int64, i32, i32,
                                             vp, vp, i32, i32, vp, vp, C.c_float, vp, vp,
                                             sz, vp, vp]
+        L.slx_paged_attn_launches.restype = i32
+        L.slx_paged_attn_launches.argtypes = []
         L.slx_logits_process.restype = i32
         L.slx_logits_process.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp, vp]
         _lib = L
@@ -665,7 +667,7 @@ def paged_append(qkv: int, stride: int, T: int, n_q: int, q_norm: int,
                                   stream)
     if rc:
         _check("slx_paged_append", rc)
-    LAUNCHES[0] += 1
+    LAUNCHES[0] += T > 0
 
 
 def paged_attn_workspace_bytes(T: int, n_q: int, n_kv: int,
@@ -677,13 +679,14 @@ def paged_attn_decode(q: int, q_stride: int, T: int, n_q: int, pages: bytes,
                       table: int, n_req: int, max_pages: int, req, pos: int,
                       scale: float, out: int, workspace: int, nbytes: int,
                       status: int, stream: int) -> None:
-    """Attention of T rows over the pages (two launches)."""
-    rc = _fast().slx_paged_attn_decode(q, q_stride, T, n_q, pages, table,
-                                       n_req, max_pages, req, pos, scale, out,
-                                       workspace, nbytes, status, stream)
+    """Attention of T rows over the pages (one to four launches)."""
+    f = _fast()
+    rc = f.slx_paged_attn_decode(q, q_stride, T, n_q, pages, table, n_req,
+                                 max_pages, req, pos, scale, out, workspace,
+                                 nbytes, status, stream)
     if rc:
         _check("slx_paged_attn_decode", rc)
-    LAUNCHES[0] += 2
+    LAUNCHES[0] += f.slx_paged_attn_launches()
 
 
 def logits_process(logits: int, f32: bool, T: int, V: int, rules: bytes, out,
@@ -693,7 +696,7 @@ def logits_process(logits: int, f32: bool, T: int, V: int, rules: bytes, out,
                                     status, stream)
     if rc:
         _check("slx_logits_process", rc)
-    LAUNCHES[0] += 1
+    LAUNCHES[0] += T > 0
 
 
 def pread_many(fds: np.ndarray, offsets: np.ndarray, sizes: np.ndarray,

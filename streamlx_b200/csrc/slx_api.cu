@@ -900,6 +900,12 @@ size_t slx_paged_attn_workspace_bytes(int T, int n_q, int n_kv, int head_dim) {
   return slx::paged_attn_workspace_bytes(T, n_q, n_kv, head_dim);
 }
 
+namespace {
+thread_local int g_attn_launches = 0;
+}
+
+int slx_paged_attn_launches(void) { return g_attn_launches; }
+
 int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
                           const slx_kv_pages* pages, const int32_t* table,
                           int n_req, int max_pages, const int32_t* req,
@@ -907,6 +913,7 @@ int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
                           void* workspace, size_t workspace_bytes,
                           int32_t* status, void* stream) {
   g_err.clear();
+  g_attn_launches = 0;
   slx::PagedAttnArgs a = {};
   const int bad = pages_ok(pages, "paged_attn", &a.kv);
   if (bad) return bad;
@@ -942,7 +949,7 @@ int slx_paged_attn_decode(const void* q, int64_t q_stride, int T, int n_q,
   a.ws = workspace;
   a.status = status;
   const int rc = slx::launch_paged_attn(a, pages->dtype == SLX_KV_E4M3,
-                                        reinterpret_cast<cudaStream_t>(stream));
+                                        reinterpret_cast<cudaStream_t>(stream), &g_attn_launches);
   return rc ? cuda_check(rc, "slx_paged_attn_decode") : SLX_OK;
 }
 

@@ -201,11 +201,13 @@ struct LogitArgs {
 int launch_paged_plan(const PlanArgs& a, cudaStream_t s);
 int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s);
 size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd);
-int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s);
+// (`launches`: goes up by one with every kernel)
+int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s, int* launches);
 int paged_tile_rows(const PagedAttnArgs& a);
 constexpr int kTileFlags = 1024;  // a call of more blocks of rows goes without
 struct TileWork;
-int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStream_t s);
+int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStream_t s,
+                      int* launches);
 size_t paged_tile_workspace_bytes(int nq, int nkv, int hd);
 int launch_logits(const LogitArgs& a, bool f32, cudaStream_t s);
 size_t prefill_scratch_bytes(int n_blocks, int H, int I);

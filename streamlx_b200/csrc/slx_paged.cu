@@ -1455,7 +1455,7 @@ size_t paged_attn_workspace_bytes(int T, int nq, int nkv, int hd) {
   return T == 0 ? 0 : attn_parts_bytes(nq, nkv, hd) + kTileFlags * sizeof(int32_t);
 }
 
-int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
+int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s, int* launches) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
   // Requests with the rows for 48 columns and more on average, and work for the
   // device: the kernel for chunks.  This one -> that: 512 rows, 24/4 heads of 128
@@ -1478,7 +1478,7 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
     tile.left = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(a.ws) +
                                            attn_parts_bytes(a.nq, nkv, a.kv.hd));
     tile.least = rest ? (31 + G) / G : 0;
-    const int rc = launch_paged_tile(a, e4m3, tile, s);
+    const int rc = launch_paged_tile(a, e4m3, tile, s, launches);
     if (rc) return rc;
     if (!rest) return SLX_OK;
   }
@@ -1516,6 +1516,7 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
   if ((rest ? launch_chained(k, dim3(grid), dim3(kPaThreads), smem, s, a, ws, rpb, tile)
             : launch_k(k, dim3(grid), dim3(kPaThreads), smem, s, a, ws, rpb, tile)) != cudaSuccess)
     return SLX_ERR_CUDA;
+  ++*launches;
   // one CTA per column while they fit the device about twice over
   const unsigned n = (unsigned)(segs <= grid ? segs : grid);
   const bool col = n * (unsigned)cols <= 1024;
@@ -1523,8 +1524,10 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s) {
                           : (col ? k_paged_join<64, true> : k_paged_join<64, false>);
   const int width = cols * (a.kv.hd / 4);
   const int threads = col || 2 * width > kJoinThreads ? kJoinThreads : 2 * width;
-  return launch_chained(j, dim3(n, col ? cols : 1), dim3(threads), 0, s, a, ws, rpb) ==
-                 cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
+  if (launch_chained(j, dim3(n, col ? cols : 1), dim3(threads), 0, s, a, ws, rpb) != cudaSuccess)
+    return SLX_ERR_CUDA;
+  ++*launches;
+  return SLX_OK;
 }
 
 }  // namespace slx

@@ -559,7 +559,8 @@ int paged_tile_rows(const PagedAttnArgs& a) {
 }
 
 // Lays out the parts behind ws.o, fills in how the rows are cut, and joins them.
-int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStream_t s) {
+int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStream_t s,
+                      int* launches) {
   const int nkv = a.kv.n_kv, G = a.nq / nkv, hd = a.kv.hd, rpb = paged_tile_rows(a);
   const int cols = rpb * G, blocks = (a.T + rpb - 1) / rpb;
   const long long items = (long long)blocks * nkv;
@@ -593,11 +594,14 @@ int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStrea
   if (launch_k(k, dim3((unsigned)(items * nsplit)), dim3(kTileThreads), smem, s, a, ws) !=
       cudaSuccess)
     return SLX_ERR_CUDA;
+  ++*launches;
   if (nsplit == 1) return SLX_OK;
   const long long warps = (long long)a.T * a.nq;
-  return launch_chained(hd == 128 ? k_paged_tile_join<128> : k_paged_tile_join<64>,
-                        dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a, ws) ==
-                 cudaSuccess ? SLX_OK : SLX_ERR_CUDA;
+  if (launch_chained(hd == 128 ? k_paged_tile_join<128> : k_paged_tile_join<64>,
+                     dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a, ws) != cudaSuccess)
+    return SLX_ERR_CUDA;
+  ++*launches;
+  return SLX_OK;
 }
 
 }  // namespace slx

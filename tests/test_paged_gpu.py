@@ -1,6 +1,7 @@
 """Batched decode over a paged KV cache against plain 64-bit restatements
 (tests/paged_cases.py): the step's plan, the append and the attention."""
 
+import ctypes
 import os
 import subprocess
 import sys
@@ -1100,3 +1101,61 @@ def test_attention_runs_of_every_length(nq, nkv, hd, dtype):
     host, dev = dev_cache(lens, nkv, hd, 16, dtype, seed=nq)
     out = check_attention(queries(len(req), nq, hd), host, dev, req, pos)
     assert all((out[r] == 0).all() for r in range(len(req)) if pos[r] < 0)
+
+
+def graph_launches(call):
+    """Kernels of one captured call."""
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        call()
+    n = ctypes.c_size_t()
+    assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(
+        ctypes.c_void_p(g.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+    return n.value
+
+
+def test_launches_are_counted():
+    """LAUNCHES moves on by the kernels that a call launches: none without
+    rows; one to four for attention."""
+    pages = torch.zeros(200, 2, 2, 16, 64, dtype=BF, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    w, inv = torch.ones(64, dtype=BF, device="cuda"), torch.ones(32, device="cuda")
+    table = torch.arange(200, **i32)
+
+    def attention(T, n_req):
+        q = torch.zeros(T, 16, 64, dtype=BF, device="cuda")
+        pos = torch.arange(T, **i32) % (T // n_req or 1)
+        req = torch.arange(T, **i32) // (T // n_req or 1)
+        t = table.view(n_req, -1)
+        return lambda: ops.paged_attention(q, pages, t, pos, req=req)
+
+    def append(T):
+        qkv = torch.zeros(T, 20 * 64, dtype=BF, device="cuda")
+        at = torch.arange(T, **i32)
+        return lambda: ops.paged_append(qkv, pages, at, at, 16, w, w, EPS, inv)
+
+    def logits(T):
+        x = torch.zeros(T, 99, device="cuda")
+        return lambda: ops.process_logits(x)
+
+    def plan(n_rows):
+        a = [torch.zeros(4, **i32), torch.zeros(4, **i32), table.view(4, -1),
+             table.clone(), torch.tensor([7], **i32)]
+        return lambda: ops.paged_plan(*a, 16, n_rows)
+
+    seen = set()
+    for name, call, most in (
+            ("no rows", attention(0, 1), 0), ("single", attention(4, 4), 2),
+            ("a chunk", attention(300, 1), 2),
+            ("a chunk in one part", attention(3200, 1), 2),
+            ("chunks", attention(300, 4), 4), ("append", append(5), 1),
+            ("no append", append(0), 0), ("logits", logits(3), 1),
+            ("no logits", logits(0), 0), ("plan", plan(4), 1),
+            ("large plan", plan(5000), 1)):
+        call()
+        before = L.LAUNCHES[0]
+        call()
+        n = L.LAUNCHES[0] - before
+        assert n == graph_launches(call) <= most, name
+        seen.add(n)
+    assert seen >= {0, 1, 2, 4}
