@@ -24,6 +24,8 @@ from . import ops
 
 MAX_BIAS = 8191         # biased ids of a request
 MAX_HISTORY = 262143    # tokens of a request with penalties
+MAX_REQUESTS = 8192     # places of a cache
+MAX_TOKENS = 1 << 30    # of a request; of a cache's pages: below 2^31
 
 
 @dataclass
@@ -68,8 +70,27 @@ class PagedKVCache:
                  device=None):
         if page_size not in ops.PAGE_SIZES:
             raise ValueError(f"page_size {page_size}: one of {ops.PAGE_SIZES}")
-        if dtype == torch.float8_e4m3fn and kv_scale is None:
-            raise ValueError("an e4m3 cache needs kv_scale")
+        if not 1 <= max_requests <= MAX_REQUESTS or \
+                not 1 <= max_tokens <= MAX_TOKENS or n_pages < 1 or \
+                n_pages * page_size > 0x7fffffff:
+            raise ValueError(f"{max_requests} requests of {max_tokens} tokens "
+                             f"on {n_pages} pages of {page_size}: 1 to "
+                             f"{MAX_REQUESTS} requests, 1 to {MAX_TOKENS} "
+                             "tokens, pages for fewer than 2^31")
+        if dtype == torch.float8_e4m3fn:
+            kv_scale = [] if kv_scale is None else list(kv_scale)
+            if len(kv_scale) != layers or not all(
+                    isinstance(s, torch.Tensor) and s.is_contiguous() and
+                    s.dtype == torch.float32 and s.shape == (2, kv_heads)
+                    for s in kv_scale):
+                raise ValueError("an e4m3 cache needs kv_scale, contiguous "
+                                 f"float32 [2, {kv_heads}] for each of "
+                                 f"{layers} layers")
+            kv_scale = [s.to(device) for s in kv_scale]
+        elif dtype != torch.bfloat16:
+            raise ValueError(f"cache dtype {dtype}: bfloat16 or float8_e4m3fn")
+        elif kv_scale is not None:
+            raise ValueError("a bfloat16 cache takes no kv_scale")
         self.page_size, self.n_pages = page_size, n_pages
         self.pages = [torch.zeros(n_pages, 2, kv_heads, page_size, head_dim,
                                   dtype=dtype, device=device)

@@ -94,3 +94,31 @@ def test_failed_generate_takes_its_requests_back():
     with pytest.raises(RuntimeError):
         dec.generate([[1]], 2)          # not beside submitted ones
     assert [r.rid for r in dec._queue] == [rid]
+
+
+@pytest.mark.parametrize("kw", [
+    dict(max_requests=8193), dict(n_pages=0), dict(n_pages=1 << 27),
+    dict(max_tokens=(1 << 30) + 1), dict(cache_dtype=torch.float16),
+    dict(kv_scale=[torch.ones(2, 2)] * 2),              # bf16 pages have none
+    *[dict(cache_dtype=torch.float8_e4m3fn, kv_scale=s) for s in (
+        [torch.ones(2, 2)], torch.ones(2, 2), [torch.ones(2, 3)] * 2,
+        [torch.ones(2, 2).double()] * 2, [torch.ones(2, 4)[:, ::2]] * 2,
+        [None] * 2)]])
+def test_caches_that_no_step_could_use(kw):
+    """Refused with the decoder, not by the first step, which would lose the
+    requests; nothing is allocated before."""
+    with pytest.raises(ValueError):
+        decoder(**kw)
+
+
+def test_e4m3_caches():
+    two = [torch.ones(2, 2)] * 2
+    dec = decoder(cache_dtype=torch.float8_e4m3fn, kv_scale=two)
+    assert dec.cache.kv_scale == two
+    one = torch.full((2, 2, 2), 0.5)                    # a layer each
+    dec = decoder(cache_dtype=torch.float8_e4m3fn, kv_scale=one)
+    assert [s.tolist() for s in dec.cache.kv_scale] == one.tolist()
+    dec = decoder(cache_dtype=torch.float8_e4m3fn)
+    for s in dec.cache.kv_scale:
+        assert s[0].tolist() == pytest.approx([8 / 448] * 2)
+        assert s[1].tolist() == [1, 1]
