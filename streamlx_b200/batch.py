@@ -24,6 +24,7 @@ from . import ops
 
 MAX_BIAS = 8191         # biased ids of a request
 MAX_HISTORY = 262143    # tokens of a request with penalties
+MAX_ROWS = 65535        # of a step: what the embedding and the router take
 MAX_REQUESTS = 8192     # places of a cache
 MAX_TOKENS = 1 << 30    # of a request; of a cache's pages: below 2^31
 
@@ -256,13 +257,16 @@ class BatchDecoder:
 
     def _rows_of_slots(self) -> list[int]:
         """Rows of each slot's request in the next step (-1: its pages go
-        back)."""
+        back); chunks of later slots are cut where they pass MAX_ROWS."""
         n = []
+        spare = MAX_ROWS - sum(r is not None for r in self.slots)
         for s, r in enumerate(self.slots):
             if r is None:
                 n.append(-1 if s in self._gone else 0)
             else:
-                n.append(min(max(len(r.prompt) - r.fed, 1), self.chunk))
+                more = min(len(r.prompt) - r.fed, self.chunk) - 1
+                n.append(1 + max(0, min(more, spare)))
+                spare -= n[-1] - 1
         return n
 
     def _masks(self, counts) -> dict:

@@ -122,3 +122,21 @@ def test_e4m3_caches():
     for s in dec.cache.kv_scale:
         assert s[0].tolist() == pytest.approx([8 / 448] * 2)
         assert s[1].tolist() == [1, 1]
+
+
+def test_rows_of_a_step(monkeypatch):
+    """Prompt chunks are cut where a step would have more rows than it can;
+    every running request keeps its own."""
+    monkeypatch.setattr(batch, "MAX_ROWS", 12, raising=False)
+    dec = decoder(max_requests=4)
+    for n in (7, 9, 1, 9):
+        dec.submit([1] * n, 5)
+    dec._admit()
+    assert dec._rows_of_slots() == [7, 3, 1, 1]
+    dec.slots[0].fed = 7                    # decodes
+    assert dec._rows_of_slots() == [1, 9, 1, 1]
+    dec.slots[2] = None
+    assert dec._rows_of_slots() == [1, 9, 0, 2]
+    dec._gone.add(2)
+    dec.chunk = 4
+    assert dec._rows_of_slots() == [1, 4, -1, 4]

@@ -268,3 +268,17 @@ def test_generate_after_a_failed_one(tiny):
         assert dec.generate(prompts, 6) == want
     assert int(dec.cache.n_free.item()) == dec.cache.n_pages
     reader.close()
+
+
+def test_more_prompt_rows_than_a_step_takes(tiny):
+    """64 prompts of 1040 tokens fed at once: 66560 rows, in two steps."""
+    cfg, model, reader = load(tiny["tiny_dec"])
+    rng = np.random.default_rng(13)
+    prompts = [rng.integers(0, cfg.vocab, 1040).tolist() for _ in range(64)]
+    dec = BatchDecoder(model, max_requests=64, max_tokens=1041, page_size=64,
+                       prompt_chunk=2000)
+    for p in prompts:
+        dec.submit(p, 1)
+    got = [len(dec.step()), len(dec.step())]
+    assert sum(got) == 64 and got[1] > 0 and not dec.busy
+    reader.close()
