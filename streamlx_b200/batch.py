@@ -188,7 +188,8 @@ class BatchDecoder:
         values keep scale 1."""
         kv, hd = self.cfg.kv_heads, self.cfg.head_dim
         s = torch.ones(2, kv, device=self.device)
-        s[0] = layer.k_norm.float().abs().max() * hd ** 0.5 / 448
+        most = layer.k_norm.float().abs().max() * hd ** 0.5 / 448
+        s[0] = torch.where(most > 0, most, 1.0)     # (keys of zero)
         return s
 
     # ------------------------------------------------------------ requests --

@@ -140,3 +140,12 @@ def test_rows_of_a_step(monkeypatch):
     dec._gone.add(2)
     dec.chunk = 4
     assert dec._rows_of_slots() == [1, 4, -1, 4]
+
+
+def test_keys_without_a_weight():
+    """A key norm of zeros has keys of zero: any scale but 0 holds them."""
+    cfg_layers = decoder().model.layers
+    cfg_layers[1].k_norm = torch.zeros(64)
+    dec = decoder()
+    scale = dec._key_scale(cfg_layers[1])
+    assert (scale > 0).all() and torch.isfinite(scale).all()
