@@ -47,7 +47,7 @@ class LogitRules:
     def check(self, vocab: int, tokens: int) -> None:
         """Raise ValueError unless a request of ``tokens`` tokens can have
         these rules."""
-        if not self.repetition > 0:
+        if not np.float32(self.repetition) > 0:     # (what the kernel has)
             raise ValueError(f"repetition {self.repetition}: must be positive")
         if self.frequency != self.frequency or self.presence != self.presence:
             raise ValueError("frequency and presence must be numbers")
@@ -57,7 +57,8 @@ class LogitRules:
         if len(self.bias) > MAX_BIAS:
             raise ValueError(f"{len(self.bias)} biases: {MAX_BIAS} at most")
         for i, v in self.bias.items():
-            if not 0 <= i < vocab or v != v:
+            if not isinstance(i, (int, np.integer)) or \
+                    not 0 <= i < vocab or v != v:
                 raise ValueError(f"bias {v} of id {i} (vocabulary {vocab})")
 
 

@@ -149,3 +149,14 @@ def test_keys_without_a_weight():
     dec = decoder()
     scale = dec._key_scale(cfg_layers[1])
     assert (scale > 0).all() and torch.isfinite(scale).all()
+
+
+@pytest.mark.parametrize("rules", [
+    LogitRules(repetition=1e-50), LogitRules(bias={1.5: 1.0}),
+    LogitRules(bias={"1": 1.0})])
+def test_rules_as_the_kernel_has_them(rules):
+    """A repetition that is 0 in 32 bits, ids that are not whole numbers."""
+    dec = decoder()
+    with pytest.raises(ValueError):
+        dec.submit([1, 2], 3, rules)
+    assert idle(dec)
