@@ -1159,3 +1159,74 @@ def test_launches_are_counted():
         assert n == graph_launches(call) <= most, name
         seen.add(n)
     assert seen >= {0, 1, 2, 4}
+
+
+def as_single_rows(q, dev, req, pos):
+    """The same rows as requests of one row each (the kernel for them)."""
+    rows = torch.tensor(req).clamp(0, dev[2].shape[0] - 1).cuda()
+    return run_attention(q, (dev[0], dev[1], dev[2][rows].contiguous()), None,
+                         pos)[0]
+
+
+def close_rows(out, one):
+    """Both within their bound of the formula: half a bf16 step each, and what
+    the weights' two parts and fp32 sums leave of the row's size."""
+    lim = 2.0 ** -7 * one.abs() + 1e-3 * one.abs().amax(-1, keepdim=True)
+    return ((out.float() - one.float()).abs() <= lim + 1e-4).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_more_blocks_than_flags(dtype):
+    """Thousands of short requests, some with one row: more blocks of rows than
+    the two kernels have flags for."""
+    g = np.random.default_rng(5)
+    each = [int(n) for n in g.choice([1, 3, 5, 8], 1300)]
+    lens = [n + int(g.integers(0, 40)) for n in each]
+    host, dev = dev_cache(lens, 1, 64, 16, dtype, seed=31)
+    req, pos = chunk_rows(lens, [n - r for n, r in zip(lens, each)])
+    rows = len(req) // len(lens)
+    assert rows * 16 >= 48 and -(-len(req) // min(rows, 8)) > 1024
+    q = queries(len(req), 16, 64)
+    out, st = run_attention(q, dev, req, pos)
+    assert st == 0 and close_rows(out, as_single_rows(q, dev, req, pos))
+
+
+@pytest.mark.parametrize("pdl", [False, True])
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_mixed_calls_again(dtype, pdl):
+    """Calls of chunks beside single tokens that share a workspace, one behind
+    the other, eagerly and in a graph: the same bits every time, with and
+    without dependent launches."""
+    lens = [900, 40, 3000, 700, 1, 2000]
+    each = [120, 1, 64, 1, 1, 2]
+    host, dev = dev_cache(lens, 2, 128, 16, dtype, seed=32)
+    pages, sc, table = dev
+    plans = []
+    for back in (0, 1):                     # two calls of other rows
+        req, pos = chunk_rows(lens, [n - r for n, r in zip(lens, each)])
+        pos = [p if i % 7 or not back else -1 for i, p in enumerate(pos)]
+        q = queries(len(req), 16, 128, seed=back)
+        want = check_attention(q, host, dev, req, pos)
+        plans.append((q.cuda(), torch.tensor(req, dtype=torch.int32).cuda(),
+                      torch.tensor(pos, dtype=torch.int32).cuda(),
+                      want.cuda()))
+    ws = ops.paged_workspace(len(req), 16, 2, 128, "cuda")
+
+    def calls():
+        return [ops.paged_attention(q, pages, table, p, req=r, kv_scale=sc,
+                                    workspace=ws) for q, r, p, _ in plans * 4]
+
+    prev = L.set_pdl(pdl)
+    try:
+        eager = calls()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            captured = calls()
+        for _ in range(5):
+            g.replay()
+        torch.cuda.synchronize()
+    finally:
+        L.set_pdl(prev)
+    for outs in (eager, captured):
+        assert all(torch.equal(o, p[3]) for o, p in zip(outs, plans * 4))
+    ops.check_status(torch.device("cuda", torch.cuda.current_device()))
