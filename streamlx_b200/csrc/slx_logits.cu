@@ -154,13 +154,13 @@ SLX_DEV void warp_best(uint64_t& key, int& id) {
 // depend on the rounding of an intermediate.  Bound for a batch by those
 // phases, one behind the other in the two CTAs that an SM holds (the words'
 // shared memory, 64 registers a thread): 38 % of the issue slots, DRAM at a
-// quarter; 128 rows of 151936 in bf16 with 8000 past tokens each, cold: 63 us,
-// 70 before the logits were asked for ahead of the mask and the list held its
-// values.  A bitmap of touched ids with counts for those alone (a quarter of
-// the shared memory, four CTAs of 256 threads) goes over the history twice:
-// 90 us; the history split over the cluster, counted by atomics into the other
-// CTAs' shared memory: 80 us.  For one row by the chain history -> words ->
-// copy -> list -> cluster reduction.
+// quarter; 128 rows of 151936 with 8000 past tokens each and every rule: 51 us in
+// bf16 in a graph (59 with an emptied L2), 76 in fp32, whose ids take two passes
+// over the history.  Beside 52 us in a graph: a bitmap of touched ids with counts
+// for those alone (a quarter of the shared memory, four CTAs of 256 threads),
+// which goes over the history twice, 80; the history split over the cluster,
+// counted by atomics into the other CTAs' shared memory, 69.  For one row by the
+// chain history -> words -> copy -> list -> cluster reduction.
 template <typename T>
 __global__ void __cluster_dims__(kLogitCluster, 1, 1)
     __launch_bounds__(kLogitThreads, 2) k_logits(const LogitArgs a) {

@@ -234,8 +234,11 @@ SLX_DEV uint32_t f32x4_to_e4m3(const float (&x)[4]) {
 // (the angle in turns, in fp64, less its whole turns).  Keys of e4m3 pages go
 // through fp64 up to their one rounding: with a step of 2^-3, a value that
 // fp32 leaves on the wrong side of a step's middle would be off by far more
-// than fp32's own error.  Bound by instruction issue for many rows, by the
-// chain position -> rotations -> barrier -> stores for few.
+// than fp32's own error.  Bound by each row's chain position -> rotations ->
+// barrier -> stores; of many rows 37 % of an SM's warps are there to cover it (64
+// registers a thread), and 47 % of the issue slots are taken: 4096 rows, 16/2
+// heads of 128, in a graph: 15.2 us in e4m3, 10.6 in bf16 (6.1 and 6.4 us of
+// bytes).
 constexpr int kAppendThreads = 128;
 constexpr int kAppendAhead = 4;  // passes over the heads requested together
 
@@ -406,13 +409,15 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // fragments are chosen so that each is 16 contiguous bytes of a key.
 //   bf16: keys and values go from global memory to fragments without shared
 //   memory, the next unit's into the registers that this one's have just left
-//   (478 us for 256 requests of 6k tokens, 24/4 heads, 6.9 TB/s; through the
-//   ring below 499).
+//   (256 requests of 6k tokens, 24/4 heads, in a graph: 473 to 482 us by the
+//   machine, 6.8 to 6.95 TB/s, where a copy's reads and writes reach 6.5; through
+//   the ring below 499).
 //   e4m3: half the bytes and twice the work per byte.  A unit's keys and its
 //   values are one contiguous block each: every warp has a ring of stages in
 //   shared memory that its first lane fills by bulk copies, some units ahead
-//   and across the ends of rows (111 us for 128 requests of 1k to 16k tokens,
-//   16/2 heads; with register loads 134).
+//   and across the ends of rows (128 requests of 1k to 16k tokens, 16/2 heads, in
+//   a graph: 108 to 121 us by the machine; with register loads 134 where this
+//   took 111).
 // V pairs two keys per register (byte permutes); S^T's accumulators become
 // P^T's operand by movmatrix.
 //
@@ -428,7 +433,7 @@ int launch_paged_append(const AppendArgs& a, bool e4m3, cudaStream_t s) {
 // gets an equal share of the list (row group, kv head, unit), whatever the
 // rows' lengths.  A segment, the units of one (group, kv head), weighs
 // kPaSwitch units more than it has, about what the change to it costs (64
-// requests of 0 to 4k tokens: 51 us, 59 without).  A segment that one CTA
+// requests of 0 to 4k tokens, in a graph: 51 us, 59 without).  A segment that one CTA
 // covers is written directly, the others leave (max, sum, O) parts that
 // k_paged_join adds in order.
 
@@ -1459,7 +1464,7 @@ int launch_paged_attn(const PagedAttnArgs& a, bool e4m3, cudaStream_t s, int* la
   const int nkv = a.kv.n_kv, G = a.nq / nkv;
   // Requests with the rows for 48 columns and more on average, and work for the
   // device: the kernel for chunks.  This one -> that: 512 rows, 24/4 heads of 128
-  // in bf16, chunks of 8: 215 -> 109 us; 64 rows, 16/2, chunks of 8: 25 -> 17.
+  // in bf16, chunks of 8: 215 -> 115 us; 64 rows, 16/2, chunks of 8: 25 -> 22.
   // Not so for 32 columns (512 rows in chunks of 32, 8/8 heads of 64: 42 -> 53)
   // or 256 in all (16 rows, 16/2: 16 -> 21).
   //

@@ -16,8 +16,9 @@ namespace slx {
 // the bits that they have in the kernel for single tokens.  For bf16 pages O is
 // scaled only when a column's maximum has grown by 2^8 (P and the sum stay far
 // inside bf16's and fp32's range until then); for e4m3 pages whenever it grows,
-// because P takes all of fp16's range (8/8 heads of 64, 512 rows in chunks of 64:
-// 37 us; 34 with 2^8 of it left for growth, where weights below 2^-32 are lost).
+// because P takes all of fp16's range (8/8 heads of 64, 512 rows in chunks of 64,
+// this kernel alone: 37 us; 34 with 2^8 of the range left for growth, where weights
+// below 2^-32 are lost).
 // K and V lie in shared memory as their pages have them, rows of
 // 64 dims swizzled over 128 bytes: K-major for S, and for P V with the dims
 // inside (the descriptor's other order), so neither is transposed.  E4m3 keys
@@ -33,10 +34,11 @@ namespace slx {
 // Bound by the chain of the warps that bring the keys: 2800 cycles a tile (loads
 // issued 1100, stores and fence 450, the pair's barrier 600, eight MMAs 500;
 // the softmax takes 1900), 2400 with two CTAs on an SM; in e4m3 the conversion
-// is in it, too.  4096 rows in chunks of 512 over 4k to 8k keys, 16/2
-// heads of 128: 411 us in bf16 (about 470 TFLOP/s without P's second part), 483 in
-// e4m3; 2214 by the kernel for single tokens.  P through shared memory and one
-// place for K and V: 475; values transposed on the way to a K-major operand: 843.
+// is in it, too, and O is scaled more often.  4096 rows in chunks of 512 over 4k
+// to 8k keys, 16/2 heads of 128, in a graph: 417 us in bf16 (about 465 TFLOP/s
+// without P's second part), 514 in e4m3, 5 us of each for the kernel behind this
+// one; 2214 by the kernel for single tokens.  P through shared memory and one place
+// for K and V: 475; values transposed on the way to a K-major operand: 843.
 constexpr int kTileM = 128;       // columns (row, q head): the MMAs' M
 constexpr int kTileKeys = 64;     // keys per tile
 constexpr int kTileThreads = 256;
@@ -567,7 +569,7 @@ int launch_paged_tile(const PagedAttnArgs& a, bool e4m3, TileWork& ws, cudaStrea
   if (items > 0x7fffffff / kTileSplits) return SLX_ERR_UNSUPPORTED;
   // splits of four tiles and more in the longest request up to two CTAs per SM,
   // of two up to one (64 rows over 600 keys, 24/4 heads: 20 -> 17 us; 320 rows over
-  // 200 to 1500, 8/8, has the four: 19, by two 21)
+  // 200 to 1500, 8/8, has the four: 19 by this kernel alone, by two 21)
   const long long tiles = ((long long)a.max_pages * a.kv.page_size + kTileKeys - 1) / kTileKeys;
   auto splits = [&](int ctas, int least) {
     const long long n = std::min(ctas / items, tiles / least);

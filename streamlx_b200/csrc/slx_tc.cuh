@@ -1,5 +1,5 @@
-// 5th-generation tensor cores: TMEM, tcgen05.mma with both operands in shared
-// memory, its descriptors and barriers.
+// 5th-generation tensor cores: TMEM, tcgen05.mma with its operands in shared
+// memory or the first one in TMEM, descriptors and barriers.
 #pragma once
 #include "slx_common.cuh"
 
