@@ -1230,3 +1230,24 @@ def test_attention_mixed_calls_again(dtype, pdl):
     for outs in (eager, captured):
         assert all(torch.equal(o, p[3]) for o, p in zip(outs, plans * 4))
     ops.check_status(torch.device("cuda", torch.cuda.current_device()))
+
+
+@pytest.mark.parametrize("dtype", [BF, E4])
+def test_attention_of_a_long_document(dtype):
+    """131071 keys, one row, held to what the kernel's sums can lose: a warp of
+    its 4 x 444 adds five or six units of 16 or 32 keys, four warps and some 222
+    CTAs' parts are joined, so fewer than 512 additions stand behind a sum (the
+    bound for any order has one for every key)."""
+    n, scale = 131071, 128 ** -0.5
+    host, dev = dev_cache([n], 2, 128, 64, dtype, seed=51, tail="zero")
+    q = queries(1, 16, 128)
+    out, st = run_attention(q, dev, None, [n - 1])
+    want, any_order = P.attention(q, *host, [0], [n - 1], 64, scale)
+    K, V = P.dense(*host, 0, n, 64)
+    p = torch.softmax(torch.einsum("kgd,kld->kgl", q[0].double().reshape(
+        2, 8, 128), K) * scale, -1)
+    A = torch.einsum("kgl,kld->kgd", p, V.abs()).reshape(1, 16, 128)
+    bound = any_order - 2 * (n - 512) * 2.0 ** -23 * A
+    err = (out.double() - want).abs()
+    assert st == 0 and (bound > 0).all()
+    assert (err <= bound).all(), float((err / bound).max())
